@@ -454,6 +454,57 @@ typedef struct {
 PM355_API size_t pm355_attn_paged_scratch(int n_tokens, int n_head, int n_head_kv, int v_pad);      /* floats; tickets: n_tokens * n_head words */
 PM355_API int pm355_attn_paged(const pm355_attn_paged_args * a, int mode, pm355_stream_t stream);
 
+/* ---- (A"') a cache held in 4 bits (prima_cpp_amd/csrc/kv4.hip, attn_kv4.hip): the reference's `-ctk q4_0 -ctv q4_0` (block_q4_0, ggml/src/ggml-common.h:161-166) on pages of 64
+ * tokens that open sequences share. A block is 32 values of a head row with one f16 scale: scale = f16(M / -8), M the value of largest magnitude (the positive one where both signs
+ * reach it, magnitudes beyond 8 * 8188 = 65504 saturate), code = rint(x / scale) clamped to -8 .. 7 (halves to even), stored + 8; the value it stands for is f16(scale * code). A row
+ * (one token, one KV head) that holds a NaN or an infinity reads back as NaN. d = head_dim = 32 nb is 64, 96, 128, 192 or 256. A page holds for each KV head, one after another:
+ *   key codes    [64 tokens][4 g][nb s][4 bytes]: the 8 dimensions from 32 s + 8 g on; byte b has dimension {0, 4, 1, 5}[b] in its low and that + 2 in its high half
+ *   key scales   [64 tokens][nb]
+ *   value codes  [16 quads of tokens][16 n][nb w][4 bytes]: byte b has token {0, 2, 1, 3}[b] of the quad, dimension 32 w + n in its low and 32 w + 16 + n in its high half
+ *   value scales [nb][64 tokens]
+ * - every matrix-core operand is then a whole number of consecutive words per lane, and one token's values are bytes of their own. */
+typedef struct {
+    int32_t n_head_kv, head_dim, n_pages; void * pages;         /* [n_pages] pages of pm355_kv4_page_bytes(), 16-byte aligned */
+    const int32_t * d_table; int32_t table_ld, n_seq;           /* device [n_seq][table_ld]: page of position / 64, -1: not held */
+} pm355_kv4_cache;
+PM355_API size_t pm355_kv4_page_bytes(int n_head_kv, int head_dim);      /* 0: sizes that are not supported */
+/* Norm, rotation and cache store of new tokens in one launch (llm_build_norm on heads + ggml_rope_ext + llm_build_kv_store): per head y = x / sqrt(mean(x^2) + eps) * norm (with
+ * `norm`; norm_q / norm_k f32 [head_dim] or NULL: no weight), then the first n_rot dimensions turn by pos * d_turns[i] turns, pairs (2 i, 2 i + 1) or, with rope_neox, (i, i + n_rot / 2),
+ * times mscale. Queries go to q (type, rounded once), keys - formed in 64 bits, so that their codes depend on no order of sums - and values into the pages. A row with d_pos < 0, d_seq
+ * outside [0, n_seq), or without a page at its position stores nothing in the cache (its query is written; position 0 is taken where d_pos < 0). Rows of one call have different (sequence, position). */
+typedef struct {
+    int32_t type, n_head, n_tokens;                             /* PM355_TYPE_BF16 or F32, of proj and q; n_head a multiple of n_head_kv */
+    const void * proj; int64_t ld_proj;                         /* [n_tokens] rows [q: n_head d | k: n_head_kv d | v: n_head_kv d], ld_proj values apart (a multiple of 4, 16-byte aligned) */
+    void * q; int64_t ldq;                                      /* [n_tokens] rows of n_head d values (a multiple of 4, 16-byte aligned) */
+    int32_t norm; const float * norm_q, * norm_k; float eps;
+    const double * d_turns; int32_t n_rot, rope_neox; float mscale;      /* device [n_rot / 2] (pm355_rope_turns) or NULL: no rotation; n_rot a multiple of 8 */
+    const int32_t * d_pos, * d_seq;                             /* device [n_tokens] */
+} pm355_kv4_append_args;
+PM355_API int pm355_kv4_append(const pm355_kv4_cache * c, const pm355_kv4_append_args * a, pm355_stream_t stream);
+/* the cached keys and values of n_tokens (sequence, position) as the f16 values they stand for: k, v [n_tokens][n_head_kv][head_dim], 16-byte aligned; zeros where no page is held */
+PM355_API int pm355_kv4_load(const pm355_kv4_cache * c, const int32_t * d_pos, const int32_t * d_seq, int n_tokens, void * k, void * v, pm355_stream_t stream);
+/* Host: turns per position of each pair, freq_base^(-2 i / n_dims) / (2 pi), scaled like rope_yarn (ggml.c:14094-14131) and divided by freq_factors[i] (host, or NULL); *mscale likewise. In 64
+ * bits, so that a position of 10^6 still has its angle to 10^-9. */
+PM355_API int pm355_rope_turns(const pm355_rope_params * rp, const float * freq_factors, double * turns, float * mscale);
+/* Attention over the pages: a query at position i sees the cached keys j <= i, with window > 0 those with i - j < window or j < n_first, on pages that are held; score = scale (q . k), softmax,
+ * weighted values; 0 for a query that sees nothing (position < 0 among them). Queries come in tiles of consecutive tokens of one sequence, device int32 {row, tokens, position of the first,
+ * sequence} each, of at most tile_tokens tokens. n_head / n_head_kv * tile_tokens <= 16, or tile_tokens == 1: decoded and drafted tokens, keys split over workgroups by max_keys (the
+ * most keys that a tile sees; only the speed depends on it); up to 128: prompts. Keys and values are the cache's f16 values; queries and probabilities are f16 with type BF16 (queries
+ * scaled by a power of two per row) and pairs of f16 - 22 bits - with type F32; sums and softmax in f32. work: f32 scratch for split keys (>= pm355_attn_kv4_work_floats() lets every
+ * split happen), zeroed once, left fit for the next call, used by one call at a time; NULL: no splits. Rows that no tile names are left as they are. */
+typedef struct {
+    int32_t type, n_head; const void * q; int64_t ldq; void * out; int64_t ldo;      /* rows of n_head d values, ld a multiple of 8, 16-byte aligned */
+    float scale; int32_t window, n_first;
+    const int32_t * d_tiles; int32_t n_tiles, tile_tokens, max_keys;
+    int32_t n_tokens;                                           /* rows of q and out */
+    float * work; size_t work_floats;
+} pm355_attn_kv4_args;
+PM355_API size_t pm355_attn_kv4_work_floats(int n_head, int n_head_kv, int head_dim);
+PM355_API int pm355_attn_kv4(const pm355_kv4_cache * c, const pm355_attn_kv4_args * a, pm355_stream_t stream);
+/* Pages of a pool copied in every layer: for each (from, to) of n_pairs host pairs, pages[layer][to] = pages[layer][from], page_bytes (a multiple of 16) each, layers layer_bytes apart. Every
+ * `to` stands once and is no `from` (llama_kv_cache_seq_cp and llama_kv_cache_defrag move cells, src/llama.cpp:4183, :4334). The pairs travel with the launch. */
+PM355_API int pm355_pages_copy(void * pages, size_t page_bytes, size_t layer_bytes, int n_layers, int n_pages, const int32_t * pairs, int n_pairs, pm355_stream_t stream);
+
 /* ---- (B) engine: resident decoder for one layer window --------------------------------------------- */
 typedef struct pm355_model pm355_model;
 
@@ -544,6 +595,14 @@ PM355_API int pm355_page_pool_open(pm355_page_pool * p);                        
 PM355_API int pm355_page_pool_close(pm355_page_pool * p, int seq);
 PM355_API int pm355_page_pool_grow(pm355_page_pool * p, int seq, int n_tokens);           /* pages for positions [0, n_tokens) that are not there yet; all or nothing */
 PM355_API int pm355_page_pool_drop_before(pm355_page_pool * p, int seq, int position);    /* releases the pages that lie wholly in front of `position` */
+PM355_API int pm355_page_pool_drop(pm355_page_pool * p, int seq, int from, int to);       /* releases the pages that lie wholly in [from, to), e.g. between first tokens and window */
+/* Forked sequences share pages, which are written by one user only: own() gives `seq` pages of its own from position `from` on and writes (from, to) pairs of what pm355_pages_copy has
+ * to copy before the next append; compact() moves the pages in use to the front of the pool. Both return the number of pairs, and change nothing where an error comes back (E_RANGE: more
+ * than max_pairs, E_NOMEM: no free pages). */
+PM355_API int pm355_page_pool_fork(pm355_page_pool * p, int seq, int n_tokens);           /* a new sequence with the pages of the first n_tokens positions: its id */
+PM355_API int pm355_page_pool_own(pm355_page_pool * p, int seq, int from, int32_t * pairs, int max_pairs);
+PM355_API int pm355_page_pool_compact(pm355_page_pool * p, int32_t * pairs, int max_pairs);
+PM355_API int pm355_page_pool_users(const pm355_page_pool * p, int page);                 /* sequences that hold the page */
 PM355_API int pm355_page_pool_page(const pm355_page_pool * p, int seq, int index);
 PM355_API int pm355_page_pool_free_pages(const pm355_page_pool * p);
 

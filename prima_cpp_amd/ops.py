@@ -608,3 +608,159 @@ def attn_paged(args, mode):
 
 def attn_paged_scratch(n_tokens, n_head, n_head_kv, v_pad):
     return L.declare("pm355_attn_paged_scratch", _sz, [_i32, _i32, _i32, _i32])(n_tokens, n_head, n_head_kv, v_pad)
+
+
+# ---- a cache held in 4 bits, in pages (part A"' of the C ABI) ----------------------------------------------------------------------
+class KV4Cache(L.C.Structure):
+    _fields_ = [("n_head_kv", L.C.c_int32), ("head_dim", L.C.c_int32), ("n_pages", L.C.c_int32), ("pages", _vp), ("d_table", _vp), ("table_ld", L.C.c_int32), ("n_seq", L.C.c_int32)]
+
+
+class KV4AppendArgs(L.C.Structure):
+    _fields_ = [("type", L.C.c_int32), ("n_head", L.C.c_int32), ("n_tokens", L.C.c_int32), ("proj", _vp), ("ld_proj", _i64), ("q", _vp), ("ldq", _i64), ("norm", L.C.c_int32), ("norm_q", _vp),
+                ("norm_k", _vp), ("eps", _f32), ("d_turns", _vp), ("n_rot", L.C.c_int32), ("rope_neox", L.C.c_int32), ("mscale", _f32), ("d_pos", _vp), ("d_seq", _vp)]
+
+
+class AttnKV4Args(L.C.Structure):
+    _fields_ = [("type", L.C.c_int32), ("n_head", L.C.c_int32), ("q", _vp), ("ldq", _i64), ("out", _vp), ("ldo", _i64), ("scale", _f32), ("window", L.C.c_int32), ("n_first", L.C.c_int32),
+                ("d_tiles", _vp), ("n_tiles", L.C.c_int32), ("tile_tokens", L.C.c_int32), ("max_keys", L.C.c_int32), ("n_tokens", L.C.c_int32), ("work", _vp), ("work_floats", _sz)]
+
+
+def _operands(*named):
+    """(name, tensor, dtypes, dimensions): what the kernels take for granted of tensors that they get as pointers - on the current device, rows whose values lie side by side"""
+    for name, t, dtypes, dims in named:
+        if t is None:
+            continue
+        if not isinstance(t, torch.Tensor) or t.device.type != "cuda" or t.device.index != torch.cuda.current_device():
+            raise L.PM355Error("%s: a tensor on the current HIP device is wanted" % name)
+        if t.dtype not in dtypes or t.dim() != dims or (t.numel() and t.stride(-1) != 1):
+            raise L.PM355Error("%s: %d dimensions of %s, the last one contiguous, are wanted" % (name, dims, " or ".join(str(d) for d in dtypes)))
+
+
+def kv4_page_bytes(n_head_kv, head_dim):
+    """bytes of a 64-token page of one layer: 4.5 bits per value"""
+    n = L.declare("pm355_kv4_page_bytes", _sz, [_i32, _i32])(n_head_kv, head_dim)
+    if not n:
+        raise L.PM355Error("head_dim is 64, 96, 128, 192 or 256: got %d heads of %d" % (n_head_kv, head_dim))
+    return n
+
+
+def _kv4_cache(pages, table, n_head_kv, head_dim):
+    _operands(("pages", pages, (torch.uint8,), 2), ("table", table, (torch.int32,), 2))
+    if pages.shape[1] != kv4_page_bytes(n_head_kv, head_dim) or not pages.is_contiguous():
+        raise L.PM355Error("pages: contiguous [pages, %d] is wanted" % kv4_page_bytes(n_head_kv, head_dim))
+    if not table.numel() or not table.is_contiguous():
+        raise L.PM355Error("table: contiguous rows of page numbers, one per sequence, are wanted")
+    return KV4Cache(n_head_kv, head_dim, pages.shape[0], ptr(pages), ptr(table), table.shape[1], table.shape[0])
+
+
+def _rows_of(name, t, n):
+    if t.shape[0] != n:
+        raise L.PM355Error("%s: %d rows are wanted, got %d" % (name, n, t.shape[0]))
+
+
+def rope_turns(n_dims, n_ctx_orig=8192, freq_base=10000.0, freq_scale=1.0, ext_factor=0.0, attn_factor=1.0, beta_fast=32.0, beta_slow=1.0, freq_factors=None):
+    """(turns, mscale): turns per position of each rotation pair, 64-bit on the current device, and the factor of kv4_append; arguments as in ggml_rope_ext, freq_factors on the host"""
+    f = L.declare("pm355_rope_turns", _i32, [_vp, _vp, _vp, _vp])
+    rp = RopeParams(n_dims, 0, n_ctx_orig, freq_base, freq_scale, ext_factor, attn_factor, beta_fast, beta_slow)
+    out, scale = np.empty(max(1, n_dims // 2)), L.C.c_float()
+    ff = None if freq_factors is None else np.ascontiguousarray(freq_factors, np.float32)
+    if ff is not None and ff.shape != (n_dims // 2,):
+        raise L.PM355Error("freq_factors: %d values are wanted" % (n_dims // 2))
+    check(f(L.C.addressof(rp), None if ff is None else ff.ctypes.data, out.ctypes.data, L.C.addressof(scale)), "rope_turns")
+    return torch.from_numpy(out).to(_dev()), scale.value
+
+
+def kv4_append(proj, pages, table, pos, seq, n_head, n_head_kv, head_dim, q=None, norm=False, norm_q=None, norm_k=None, eps=1e-6, turns=None, mscale=1.0, neox=False):
+    """Queries normed and rotated (returned, [T, n_head * head_dim] in the type of proj), keys likewise and values into 4-bit pages. proj [T, >= (n_head + 2 n_head_kv) * head_dim] rows
+    q | k | v, f32 or bf16; pages uint8 [n, kv4_page_bytes()], table int32 [sequences, pages of a sequence], pos, seq int32 [T]; turns (rope_turns): None rotates nothing."""
+    c = _kv4_cache(pages, table, n_head_kv, head_dim)
+    _operands(("proj", proj, (torch.float32, torch.bfloat16), 2), ("pos", pos, (torch.int32,), 1), ("seq", seq, (torch.int32,), 1), ("norm_q", norm_q, (torch.float32,), 1),
+              ("norm_k", norm_k, (torch.float32,), 1), ("turns", turns, (torch.float64,), 1))
+    T = proj.shape[0]
+    if q is None:
+        q = torch.empty(T, n_head * head_dim, dtype=proj.dtype, device=proj.device)
+    _operands(("q", q, (proj.dtype,), 2))
+    for name, t in (("pos", pos), ("seq", seq), ("q", q)):
+        _rows_of(name, t, T)
+    for name, t in (("norm_q", norm_q), ("norm_k", norm_k)):
+        if t is not None:
+            _rows_of(name, t, head_dim)
+            if not norm:
+                raise L.PM355Error("%s without norm=True" % name)
+    if proj.shape[1] < (n_head + 2 * n_head_kv) * head_dim or q.shape[1] < n_head * head_dim:
+        raise L.PM355Error("proj, q: rows of %d and %d values are wanted" % ((n_head + 2 * n_head_kv) * head_dim, n_head * head_dim))
+    if not T:
+        return q
+    ld = lambda t: t.stride(0) if t.shape[0] > 1 else t.shape[1] // 8 * 8  # noqa: E731
+    a = KV4AppendArgs(pm_type(proj), n_head, T, ptr(proj), ld(proj), ptr(q), ld(q), int(norm), ptr(norm_q), ptr(norm_k), float(eps), ptr(turns), 0 if turns is None else 2 * turns.numel(), int(neox),
+                      float(mscale), ptr(pos), ptr(seq))
+    f = L.declare("pm355_kv4_append", _i32, [L.C.POINTER(KV4Cache), L.C.POINTER(KV4AppendArgs), _vp])
+    check(f(L.C.byref(c), L.C.byref(a), stream_ptr()), "kv4_append")
+    return q
+
+
+def kv4_load(pages, table, pos, seq, n_head_kv, head_dim):
+    """(k, v): what the pages hold for these (sequence, position), f16 [T, n_head_kv, head_dim]"""
+    c = _kv4_cache(pages, table, n_head_kv, head_dim)
+    _operands(("pos", pos, (torch.int32,), 1), ("seq", seq, (torch.int32,), 1))
+    T = pos.shape[0]
+    _rows_of("seq", seq, T)
+    k, v = (torch.empty(T, n_head_kv, head_dim, dtype=torch.float16, device=pages.device) for _ in range(2))
+    if T:
+        f = L.declare("pm355_kv4_load", _i32, [L.C.POINTER(KV4Cache), _vp, _vp, _i32, _vp, _vp, _vp])
+        check(f(L.C.byref(c), ptr(pos), ptr(seq), T, ptr(k), ptr(v), stream_ptr()), "kv4_load")
+    return k, v
+
+
+def kv4_tiles(entries, n_head, n_head_kv):
+    """(tiles, tile_tokens, max_keys) of attn_kv4 for entries (sequence, first new position, new tokens) whose rows follow each other: int32 [n, 4] on the host, and two numbers"""
+    R, most = n_head // n_head_kv, max((n for _, _, n in entries), default=1)
+    tile = max(1, (16 if most * R <= 16 or most == 1 else 128) // R)
+    out, row = [], 0
+    for s, p, n in entries:
+        out += [(row + i, min(tile, n - i), p + i, s) for i in range(0, n, tile)]
+        row += n
+    return np.array(out, np.int32).reshape(-1, 4), tile, max((p + n for _, p, n in entries), default=0)
+
+
+def kv4_work(n_head, n_head_kv, head_dim):
+    """scratch that lets attn_kv4 split the keys of few rows over workgroups: zeroed here, for one call at a time"""
+    n = L.declare("pm355_attn_kv4_work_floats", _sz, [_i32, _i32, _i32])(n_head, n_head_kv, head_dim)
+    return torch.zeros(n, device=_dev())
+
+
+def attn_kv4(q, pages, table, tiles, tile_tokens, max_keys, n_head, n_head_kv, head_dim, scale, window=0, n_first=0, out=None, work=None):
+    """Attention of q [T, n_head * head_dim] (f32 or bf16) over 4-bit pages: causal, with window > 0 only the last `window` keys and the first n_first. tiles int32 [n, 4] {row, tokens,
+    position, sequence} (kv4_tiles). Returns out, of which the rows that tiles name are written. work: kv4_work(), for one call at a time."""
+    c = _kv4_cache(pages, table, n_head_kv, head_dim)
+    _operands(("q", q, (torch.float32, torch.bfloat16), 2), ("tiles", tiles, (torch.int32,), 2), ("work", work, (torch.float32,), 1))
+    if q.shape[1] < n_head * head_dim or tiles.shape[1] != 4 or not tiles.is_contiguous():
+        raise L.PM355Error("q, tiles: rows of %d values and contiguous rows of 4 are wanted" % (n_head * head_dim))
+    if out is None:
+        out = torch.empty(q.shape[0], n_head * head_dim, dtype=q.dtype, device=q.device)
+    _operands(("out", out, (q.dtype,), 2))
+    _rows_of("out", out, q.shape[0])
+    if out.shape[1] < n_head * head_dim:
+        raise L.PM355Error("out: rows of %d values are wanted" % (n_head * head_dim))
+    if not q.shape[0] or not tiles.shape[0]:
+        return out
+    ld = lambda t: t.stride(0) if t.shape[0] > 1 else t.shape[1] // 8 * 8  # noqa: E731
+    a = AttnKV4Args(pm_type(q), n_head, ptr(q), ld(q), ptr(out), ld(out), float(scale), window, n_first, ptr(tiles), tiles.shape[0], tile_tokens, max_keys, q.shape[0], ptr(work),
+                    0 if work is None else work.numel())
+    f = L.declare("pm355_attn_kv4", _i32, [L.C.POINTER(KV4Cache), L.C.POINTER(AttnKV4Args), _vp])
+    check(f(L.C.byref(c), L.C.byref(a), stream_ptr()), "attn_kv4")
+    return out
+
+
+def pages_copy(pages, pairs):
+    """pages[.., to] = pages[.., from] for (from, to) pairs on the host: uint8 [layers, n, page bytes] or [n, page bytes]; every `to` stands once and is no `from`"""
+    if pages.dim() == 2:
+        pages = pages[None]
+    _operands(("pages", pages, (torch.uint8,), 3))
+    if not pages[0].is_contiguous():
+        raise L.PM355Error("pages: contiguous layers are wanted")
+    pairs = np.ascontiguousarray(pairs, np.int32).reshape(-1, 2)
+    if not len(pairs):
+        return
+    f = L.declare("pm355_pages_copy", _i32, [_vp, _sz, _sz, _i32, _i32, _vp, _i32, _vp])
+    check(f(ptr(pages), pages.shape[2], pages.stride(0) if pages.shape[0] > 1 else pages[0].numel(), pages.shape[0], pages.shape[1], pairs.ctypes.data, len(pairs), stream_ptr()), "pages_copy")
