@@ -195,7 +195,7 @@ def attend_case(d, H, G, type, entries, window=0, first=0, seed=0, drop=(), spre
                     assert np.isnan(o).all() and np.isnan(e).all(), (s, i, h)
                     continue
                 tol = half * np.abs(e) + (pq[0] + 2.0 ** -18 + 2 * (d * 2.0 ** -24 + pq[1]) * B) * A + 2.0 ** -33 * np.abs(vs[g][ok].astype(np.float64)).sum(0)
-                bad = np.abs(o - e) > tol
+                bad = ~(np.abs(o - e) <= tol)
                 assert not bad.any(), (s, i, h, o[bad][:3], e[bad][:3], tol[bad][:3])
                 worst = max(worst, float((np.abs(o - e) / np.maximum(tol, 1e-30)).max()))
         row += n
