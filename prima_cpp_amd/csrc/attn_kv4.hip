@@ -1,7 +1,7 @@
 // attn_kv4.hip — attention over pages held in 4 bits: causal, with a sliding window and first tokens that stay visible.
 //
 // o = sum_j p_j v_j / sum_j p_j, p_j = exp2(cf q k_j - max), over the j that the query sees; one pass over the keys with the running maximum and sum, both products on the f16 matrix cores.
-// Keys and values become f16 in registers: a pair of codes is masked out of a word over the bits of 1024, less 1032, times the scale - 3.25 packed operations for two values (the words are
+// Keys and values become f16 in registers: a pair of codes is masked out of a word over the bits of 1024, less 1032, times the scale - 3.25 operations for two values (the words are
 // ordered so that a mask gives a pair that an operand wants). Queries are brought to [1, 2) by a power of two per row, exact for bf16; WIDE (32-bit rows) holds queries and probabilities as
 // pairs of f16 and makes two products of each. Probabilities are held times 2^8, so that f16 has its steps of 2^-11 down to p = 2^-22.
 // S^T = K Q^T is computed with the key rows permuted so that a lane's score registers are its P operand of O^T = V^T P^T.
@@ -13,6 +13,7 @@
 
 namespace {
 
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x3 __attribute__((ext_vector_type(3), aligned(4)));
@@ -38,13 +39,23 @@ template <int N> __device__ __forceinline__ void ld_halves(const char * p, uint3
     } else ld_words<N / 2>(p, w);
 }
 __device__ __forceinline__ f16x2 half_of(const uint32_t * w, int i) {      // value i of packed halves, twice
-    const uint32_t h = i & 1 ? w[i >> 1] >> 16 : w[i >> 1] & 0xffff;
-    return __builtin_bit_cast(f16x2, h | h << 16);
+    const f16x2 t = __builtin_bit_cast(f16x2, w[i >> 1]);
+    return i & 1 ? f16x2{t.y, t.y} : f16x2{t.x, t.x};
 }
-// the codes at nibble p of both halves of a word, times scales: two f16 values
-__device__ __forceinline__ f16x2 pair(uint32_t w, int p, f16x2 s) {
-    const f16x2 n = __builtin_bit_cast(f16x2, (w >> (4 * p) & 0x000f000fu) | 0x64006400u);
-    return (n - f16x2{(_Float16) 1032.0f, (_Float16) 1032.0f}) * s;
+// one operation for (w & mask) | bits: of two constants one has to sit in a vector register, which the compiler does not choose by itself (it takes two operations)
+__device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t mask, uint32_t bits) {
+    uint32_t r;
+    asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(r) : "v"(w), "s"(mask), "v"(bits));
+    return r;
+}
+// the four pairs of codes of a word, less 8: those at nibbles 0 and 2 over the bits of 1024, those at 1 and 3 are 1024 + 16 code
+__device__ __forceinline__ void codes(uint32_t w, f16x2 * n) {
+    const uint32_t u = w >> 8;
+    const f16x2 zero = {(_Float16) -1032.0f, (_Float16) -1032.0f}, part = {(_Float16) 0.0625f, (_Float16) 0.0625f}, less = {(_Float16) -72.0f, (_Float16) -72.0f};
+    n[0] = __builtin_bit_cast(f16x2, and_or(w, 0x000f000fu, 0x64006400u)) + zero;
+    n[1] = __builtin_elementwise_fma(__builtin_bit_cast(f16x2, and_or(w, 0x00f000f0u, 0x64006400u)), part, less);
+    n[2] = __builtin_bit_cast(f16x2, and_or(u, 0x000f000fu, 0x64006400u)) + zero;
+    n[3] = __builtin_elementwise_fma(__builtin_bit_cast(f16x2, and_or(u, 0x00f000f0u, 0x64006400u)), part, less);
 }
 __device__ __forceinline__ f16x8 eight(f16x2 a, f16x2 b, f16x2 c, f16x2 d) { return f16x8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y}; }
 // scales beyond what the cache store makes (8188: its codes stay finite), NaN and infinities become 0; bits 0, 1: which
@@ -53,8 +64,78 @@ __device__ __forceinline__ uint32_t finite(uint32_t & s) {
     s &= (lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u);
     return lo | hi << 1;
 }
-__device__ __forceinline__ void st_shared(float * p, float v) { __hip_atomic_store((PM_G float *) p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
-__device__ __forceinline__ float ld_shared(const float * p) { return __hip_atomic_load((const PM_G float *) p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+// ---- partial sums of split keys: per slot [splits][COLS][D] and [splits][COLS][maximum, sum]; stores that every XCD sees once they are waited for
+__device__ __forceinline__ void put(float * p, float x, float y) {
+    __hip_atomic_store((PM_G uint64_t *) p, __builtin_bit_cast(uint64_t, f32x2{x, y}), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ void put(float * p, f32x4 v) { put(p, v.x, v.y); put(p + 2, v.z, v.w); }
+// After put(): whether this workgroup is the last of its slot. Tickets count up to `splits` and go back to 0.
+__device__ __forceinline__ bool last_of(float * work, size_t slot, int splits) {
+    __shared__ int is_last;
+    pm_vm_drain();
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        unsigned * tk = (unsigned *) work + slot;
+        is_last = __hip_atomic_fetch_add(tk, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned) splits - 1;
+        if (is_last) __hip_atomic_store(tk, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    if (!is_last) return false;
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+    return true;
+}
+// The last one joins the splits in their order (results do not depend on who that is): 4 dimensions of a column per thread, up to 16 splits on their way at once - a load that comes from
+// another XCD's store takes about a microsecond, and one at a time 128 splits took 40. lds: splits * COLS * 2 + 1024 floats
+template <int D, int COLS, typename F> __device__ __forceinline__ void join(const float * part, int splits, int cols, float * lds, F && store) {
+    __shared__ float inv[COLS];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const float * ml = part + (size_t) splits * COLS * D;
+    for (int o = threadIdx.x; o < splits * COLS; o += 256)
+        if (o % COLS < cols) { const f32x2 v = *(const PM_G f32x2 *) (ml + 2 * o); lds[2 * o] = v.x; lds[2 * o + 1] = v.y; }
+    __syncthreads();
+    for (int col = wave; col < cols; col += 4) {           // maximum and sum of a column by a wave; the factors of its splits take the place of their maxima
+        float M = NONE, L = 0.0f;
+        for (int k = lane; k < splits; k += 64) M = fmaxf(M, lds[(k * COLS + col) * 2]);
+        M = all_max(M);
+        for (int k = lane; k < splits; k += 64) { const float f = __builtin_amdgcn_exp2f(lds[(k * COLS + col) * 2] - M); lds[(k * COLS + col) * 2] = f; L = fmaf(lds[(k * COLS + col) * 2 + 1], f, L); }
+        L = wave_sum(L);
+        if (lane == 0) inv[col] = L == 0.0f ? 0.0f : 1.0f / L;
+    }
+    __syncthreads();
+    const int items = cols * (D / 4), groups = items < 256 ? 256 / items : 1;
+    float * sums = lds + splits * COLS * 2;
+    for (int o = threadIdx.x; o < items * groups; o += 256) {
+        const int grp = o / items, it = o % items, col = it / (D / 4), d = it % (D / 4) * 4;
+        const float * p = part + (size_t) col * D + d;
+        f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int k0 = grp; k0 < splits; k0 += 16 * groups) {
+            f32x4 r[16];
+#pragma unroll
+            for (int k = 0; k < 16; ++k) { const int z = k0 + k * groups; r[k] = *(const PM_G f32x4 *) (p + (size_t) (z < splits ? z : splits - 1) * COLS * D); }
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+                const int z = k0 + k * groups;
+                const float f = z < splits ? lds[(z * COLS + col) * 2] : 0.0f;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) if (z < splits) v[e] = fmaf(r[k][e], f, v[e]);
+            }
+        }
+        if (groups == 1) store(col, d, v * inv[col]);
+        else *(f32x4 *) (sums + o * 4) = v;
+    }
+    if (groups == 1) return;
+    __syncthreads();
+    for (int it = threadIdx.x; it < items; it += 256) {
+        f32x4 v = *(const f32x4 *) (sums + it * 4);
+        for (int k = 1; k < groups; ++k) v += *(const f32x4 *) (sums + (k * items + it) * 4);
+        const int col = it / (D / 4);
+        store(col, it % (D / 4) * 4, v * inv[col]);
+    }
+}
+template <typename T> __device__ __forceinline__ void st_out(T * p, f32x4 v) {
+    if constexpr (sizeof(T) == 2) *(PM_G u16x4 *) p = u16x4{f2bf(v.x), f2bf(v.y), f2bf(v.z), f2bf(v.w)};
+    else *(PM_G f32x4 *) p = v;
+}
 
 // eight values of a query row as operands, times a power of two
 template <typename T> __device__ __forceinline__ void ld_query(const T * p, float * x) {
@@ -99,130 +180,152 @@ __device__ __forceinline__ int page_at(const pm_seen & s, int i) { return i < s.
 constexpr int FW = 4;                                      // waves of a workgroup
 template <int NB> struct pm_chunk { uint32_t k[2][NB], ks[2][(NB + 1) / 2], v[2][NB], vs[NB][4]; };      // codes and scales of 32 keys as a lane wants them
 
-template <typename T, int NB, bool WIDE> __global__ __launch_bounds__(FW * 64) void few_kernel(pm_kv4_cache c, pm_kv4_attn a, int splits) {
-    constexpr int D = NB * 32, VT = D / 16, LD = D + 4;
+// CT column tiles of 16 per workgroup share the keys' way from codes to f16; `passes` workgroups take the columns of a tile
+template <typename T, int NB, bool WIDE, int CT> __global__ __launch_bounds__(FW * 64, NB <= (WIDE ? 4 : 6) ? 2 : 1) void few_kernel(pm_kv4_cache c, pm_kv4_attn a, int passes, int splits) {
+    constexpr int D = NB * 32, VT = D / 16, LD = D + 4, COLS = 16 * CT;
     typedef pm_kv4_slab<NB> S;
-    extern __shared__ __attribute__((aligned(16))) float acc_l[];         // [FW][16][LD]
-    __shared__ float m_l[FW][16], l_l[FW][16], ml[64 * 32];
-    __shared__ int is_last;
-    const int G = c.G, R = a.H / G, HT = (R + 15) / 16, gh = blockIdx.x % (G * HT), g = gh / HT, ht = gh % HT, s = blockIdx.y;
+    extern __shared__ __attribute__((aligned(16))) float acc_l[];         // [FW][16][LD], then maximum and sum [splits][COLS][2]
+    __shared__ float m_l[FW][16], l_l[FW][16];
+    // (passes without columns are neighbours, not every n-th workgroup: those would leave whole XCDs idle)
+    const int G = c.G, R = a.H / G, g = blockIdx.x % G, at = blockIdx.x / G % a.n_tiles, pass = blockIdx.x / G / a.n_tiles, s = blockIdx.y;
     const size_t slot = blockIdx.x;
-    const int32_t * tile = uniform_const_ptr(a.tiles) + blockIdx.x / (G * HT) * 4;
+    const int32_t * tile = uniform_const_ptr(a.tiles) + (size_t) at * 4;
     const int row0 = tile[0], seq = tile[3], pos0 = tile[2] < 0x7fffff00 ? tile[2] : 0x7fffff00, n = tile[1] < a.tile_tokens ? tile[1] : a.tile_tokens;
-    if (n < 1) return;
+    const int col0 = pass * COLS, left = n * R - col0, cols = left < COLS ? left : COLS;
+    if (n < 1 || cols < 1) return;
     const int wave = __builtin_amdgcn_readfirstlane((int) threadIdx.x >> 6), lane = threadIdx.x & 63, lr = lane & 15, lg = lane >> 4;
-    const int nh = R <= 16 ? R : R - ht * 16 < 16 ? R - ht * 16 : 16, cols = n * nh;
-    const int ct = lr < cols ? lr / nh : 0, ch = g * R + ht * 16 + (lr < cols ? lr % nh : 0);             // token and head of this lane's column
-    const pm_seen see = seen_by(c, a, pos0, n);
-    const int pos = lr < cols && pos0 >= 0 ? pos0 + ct : -1, low = a.window > 0 ? pos - a.window + 1 : 0;
+    const int t0 = col0 / R, tn = (col0 + cols - 1) / R - t0 + 1;          // tokens of the columns
+    const pm_seen see = seen_by(c, a, pos0 < 0 ? -1 : pos0 + t0, tn);
     const int per = (see.count + splits - 1) / splits, end = 2 * ((s + 1) * per < see.count ? (s + 1) * per : see.count);
-    const int32_t * table = uniform_const_ptr(c.table) + (size_t) ((unsigned) seq < (unsigned) c.n_seq ? seq : 0) * c.table_ld;
     const bool known = (unsigned) seq < (unsigned) c.n_seq;
+    const int32_t * table = uniform_const_ptr(c.table) + (size_t) (known ? seq : 0) * c.table_ld;
     const char * head = c.pages + (size_t) g * S::BYTES;
     auto page_of = [&](int i) __attribute__((always_inline)) { if (!known || i >= end) return -1; const int p = table[page_at(see, i >> 1)]; return (unsigned) p < (unsigned) c.n_pages ? p : -1; };
-    const int krow = 8 * (lr >> 2) + (lr & 3);             // key of score row lr in the first 16 of a step (the second: + 4)
+    const uint32_t krow = 8 * (lr >> 2) + (lr & 3);        // key of score row lr in the first 16 of a step (the second: + 4)
+    const uint32_t at_k = krow * 16 * NB + lg * 4 * NB, at_ks = krow * 2 * NB, at_v = lg * 128 * NB + lr * 4 * NB, at_vs = lg * 16;
+    // (no branch around the loads: behind one the compiler waits for everything that may be on its way. What is not there is read from page 0 and left alone)
     auto load = [&](pm_chunk<NB> & x, int i, int page) __attribute__((always_inline)) {
-        if (page < 0) return;
-        const char * slab = head + (size_t) page * G * S::BYTES;
+        const char * slab = uniform_ptr((char *) head + (size_t) (page < 0 ? 0 : page) * G * S::BYTES);
         const int key = (i & 1) * 32;
+        const char * k = slab + S::K + key * 16 * NB, * ks = slab + S::KS + key * 2 * NB, * v = slab + S::V + key * 16 * NB, * vs = slab + S::VS + key * 2;
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
-            ld_words<NB>(slab + S::K + (key + krow + 4 * b) * 16 * NB + lg * 4 * NB, x.k[b]);
-            ld_words<NB>(slab + S::V + ((key >> 2) + 2 * lg + b) * 64 * NB + lr * 4 * NB, x.v[b]);
-            ld_halves<NB>(slab + S::KS + (key + krow + 4 * b) * 2 * NB, x.ks[b]);
+            ld_words<NB>(k + at_k + b * 64 * NB, x.k[b]);
+            ld_words<NB>(v + at_v + b * 64 * NB, x.v[b]);
+            ld_halves<NB>(ks + at_ks + b * 8 * NB, x.ks[b]);
         }
 #pragma unroll
-        for (int w = 0; w < NB; ++w) ld_words<4>(slab + S::VS + (w * PM_PAGE + key + 8 * lg) * 2, x.vs[w]);
+        for (int w = 0; w < NB; ++w) ld_words<4>(vs + at_vs + w * PM_PAGE * 2, x.vs[w]);
     };
     int i = 2 * s * per + wave, page = page_of(i), next = page_of(i + FW);
     pm_chunk<NB> x0, x1;
     load(x0, i, page);
 
-    f16x8 qh[NB], ql[NB];
-    float cf;
-    {
-        const int row = row0 + ct;
-        const bool on = lr < cols && (unsigned) row < (unsigned) a.n_tokens;
+    f16x8 qh[CT][NB], ql[WIDE ? CT : 1][NB];
+    f32x4 acc[CT][VT];
+    float cf[CT], m[CT], l[CT];
+    int pos[CT];
+#pragma unroll
+    for (int u = 0; u < CT; ++u) {
+        const int col = u * 16 + lr, tok = (col0 + col) / R, row = row0 + tok, h = g * R + (col0 + col) % R;
+        const bool on = col < cols && (unsigned) row < (unsigned) a.n_tokens;
+        pos[u] = col < cols && pos0 >= 0 ? pos0 + tok : -1;
         float x[NB][8], most = 0.0f;
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) x[b][j] = 0.0f;
-            if (on) ld_query<T>((const T *) a.q + (size_t) row * a.ldq + ch * D + b * 32 + lg * 8, x[b]);
+            if (on) ld_query<T>((const T *) a.q + (size_t) row * a.ldq + h * D + b * 32 + lg * 8, x[b]);
 #pragma unroll
             for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(x[b][j]));
         }
         most = fmaxf(most, __shfl_xor(most, 16)); most = fmaxf(most, __shfl_xor(most, 32));
-        const float f = row_factor(most, a.scale, cf);
+        const float f = row_factor(most, a.scale, cf[u]);
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) x[b][j] *= f;
-            split_f16(x[b], qh[b], ql[b]);
+            f16x8 lo;
+            split_f16(x[b], qh[u][b], lo);
+            if (WIDE) ql[u][b] = lo;
         }
-    }
-    f32x4 acc[VT];
 #pragma unroll
-    for (int t = 0; t < VT; ++t) acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    float m = NONE, l = 0.0f;
+        for (int t = 0; t < VT; ++t) acc[u][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        m[u] = NONE; l[u] = 0.0f;
+    }
     auto step = [&](pm_chunk<NB> & x, int i) __attribute__((always_inline)) {
-        const int key0 = page_at(see, i >> 1) * PM_PAGE + (i & 1) * 32 + lg * 8;      // the lane's eight keys
-        f32x4 s0 = {0.0f, 0.0f, 0.0f, 0.0f}, s1 = s0;
+        const int k0 = page_at(see, i >> 1) * PM_PAGE + (i & 1) * 32, key0 = k0 + lg * 8;      // the lane's eight keys
+        f32x4 s0[CT], s1[CT];
+#pragma unroll
+        for (int u = 0; u < CT; ++u) s0[u] = s1[u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
             const f16x2 sa = half_of(x.ks[0], b), sb = half_of(x.ks[1], b);
-            const f16x8 ka = eight(pair(x.k[0][b], 0, sa), pair(x.k[0][b], 1, sa), pair(x.k[0][b], 2, sa), pair(x.k[0][b], 3, sa));
-            const f16x8 kb = eight(pair(x.k[1][b], 0, sb), pair(x.k[1][b], 1, sb), pair(x.k[1][b], 2, sb), pair(x.k[1][b], 3, sb));
-            s0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qh[b], s0, 0, 0, 0);
-            s1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(kb, qh[b], s1, 0, 0, 0);
-            if (WIDE) { s0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, ql[b], s0, 0, 0, 0); s1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(kb, ql[b], s1, 0, 0, 0); }
-        }
-        float f[8];
+            f16x2 na[4], nb[4];
+            codes(x.k[0][b], na); codes(x.k[1][b], nb);
+            const f16x8 ka = eight(na[0] * sa, na[1] * sa, na[2] * sa, na[3] * sa), kb = eight(nb[0] * sb, nb[1] * sb, nb[2] * sb, nb[3] * sb);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] = j < 4 ? s0[j & 3] : s1[j & 3];
+            for (int u = 0; u < CT; ++u) {
+                s0[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qh[u][b], s0[u], 0, 0, 0);
+                s1[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kb, qh[u][b], s1[u], 0, 0, 0);
+                if (WIDE) { s0[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, ql[u][b], s0[u], 0, 0, 0); s1[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kb, ql[u][b], s1[u], 0, 0, 0); }
+            }
+        }
         // a step that not every column sees whole: hidden keys count nothing, whatever their slots hold
-        const int k0 = key0 - lg * 8;
-        if (k0 + 31 > see.lo || (a.window > 0 && k0 <= see.hi - a.window)) {
-            uint32_t bad = 0;
+        const bool whole = k0 + 31 <= see.lo && !(a.window > 0 && k0 <= see.hi - a.window);
+        uint32_t bad = 0;
+        if (!whole)
 #pragma unroll
             for (int w = 0; w < NB; ++w)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) bad |= finite(x.vs[w][j]) << 2 * j;
+        f16x8 ph[CT], pl[CT];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int key = key0 + j;
-                const bool ok = key <= pos && (key >= low || key < a.first);
-                f[j] = ok ? (bad >> j & 1 ? NAN : f[j]) : -INFINITY;
+        for (int u = 0; u < CT; ++u) {
+            float f[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) f[j] = j < 4 ? s0[u][j & 3] : s1[u][j & 3];
+            if (!whole) {
+                const int low = a.window > 0 ? pos[u] - a.window + 1 : 0;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int key = key0 + j;
+                    const bool ok = key <= pos[u] && (key >= low || key < a.first);
+                    f[j] = ok ? (bad >> j & 1 ? NAN : f[j]) : -INFINITY;
+                }
             }
+            float mx = f[0];
+#pragma unroll
+            for (int j = 1; j < 8; ++j) mx = fmaxf(mx, f[j]);
+            mx = fmaxf(mx, __shfl_xor(mx, 16)); mx = fmaxf(mx, __shfl_xor(mx, 32));
+            mx = fmaxf(mx * cf[u], NONE);
+            if (__any(mx > m[u])) {
+                const float mn = fmaxf(m[u], mx), corr = __builtin_amdgcn_exp2f(m[u] - mn);
+                m[u] = mn; l[u] *= corr;
+#pragma unroll
+                for (int t = 0; t < VT; ++t)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[u][t][e] *= corr;
+            }
+            const float mo = HELD - m[u];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) { f[j] = __builtin_amdgcn_exp2f(fmaf(f[j], cf[u], mo)); l[u] += f[j]; }
+            split_f16(f, ph[u], pl[u]);
         }
-        float mx = f[0];
-#pragma unroll
-        for (int j = 1; j < 8; ++j) mx = fmaxf(mx, f[j]);
-        mx = fmaxf(mx, __shfl_xor(mx, 16)); mx = fmaxf(mx, __shfl_xor(mx, 32));
-        mx = fmaxf(mx * cf, NONE);
-        if (__any(mx > m)) {
-            const float mn = fmaxf(m, mx), corr = __builtin_amdgcn_exp2f(m - mn);
-            m = mn; l *= corr;
-#pragma unroll
-            for (int t = 0; t < VT; ++t)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) acc[t][e] *= corr;
-        }
-        f16x8 ph, pl;
-        const float mo = HELD - m;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) { f[j] = __builtin_amdgcn_exp2f(fmaf(f[j], cf, mo)); l += f[j]; }
-        split_f16(f, ph, pl);
 #pragma unroll
         for (int w = 0; w < NB; ++w) {
-            f16x2 sc[4];
+            f16x2 sc[4], na[4], nb[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) sc[j] = __builtin_bit_cast(f16x2, x.vs[w][j]);
+            codes(x.v[0][w], na); codes(x.v[1][w], nb);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const f16x8 v = eight(pair(x.v[0][w], h, sc[0]), pair(x.v[0][w], h + 2, sc[1]), pair(x.v[1][w], h, sc[2]), pair(x.v[1][w], h + 2, sc[3]));
-                acc[2 * w + h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph, acc[2 * w + h], 0, 0, 0);
-                if (WIDE) acc[2 * w + h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl, acc[2 * w + h], 0, 0, 0);
+                const f16x8 v = eight(na[h] * sc[0], na[h + 2] * sc[1], nb[h] * sc[2], nb[h + 2] * sc[3]);
+#pragma unroll
+                for (int u = 0; u < CT; ++u) {
+                    acc[u][2 * w + h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[u], acc[u][2 * w + h], 0, 0, 0);
+                    if (WIDE) acc[u][2 * w + h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl[u], acc[u][2 * w + h], 0, 0, 0);
+                }
             }
         }
     };
@@ -235,71 +338,49 @@ template <typename T, int NB, bool WIDE> __global__ __launch_bounds__(FW * 64) v
         if (next >= 0) step(x1, i + FW);
         page = after; next = then;
     }
-    l += __shfl_xor(l, 16); l += __shfl_xor(l, 32);
-    if (lr < cols) {
-#pragma unroll
-        for (int t = 0; t < VT; ++t) *(f32x4 *) (acc_l + (wave * 16 + lr) * LD + t * 16 + lg * 4) = acc[t];
-        if (lg == 0) { m_l[wave][lr] = m; l_l[wave][lr] = l; }
-    }
-    __syncthreads();
-    auto store = [&](int col, int d, float o) {
-        const int row = row0 + col / nh;
-        if ((unsigned) row < (unsigned) a.n_tokens) ((T *) a.out)[(size_t) row * a.ldo + (g * R + ht * 16 + col % nh) * D + d] = from_f<T>(o);
+    auto store = [&](int col, int d, f32x4 o) {
+        const int row = row0 + (col0 + col) / R;
+        if ((unsigned) row < (unsigned) a.n_tokens) st_out((T *) a.out + (size_t) row * a.ldo + (g * R + (col0 + col) % R) * D + d, o);
     };
-    float * part = a.work + TICKETS + slot * splits * 16 * (D + 2);
-    for (int o = threadIdx.x; o < cols * D; o += FW * 64) {
-        const int col = o / D, d = o % D;
-        float M = NONE, v = 0.0f, sum = 0.0f;
+    float * part = a.work + TICKETS + slot * splits * COLS * (D + 2);
 #pragma unroll
-        for (int w = 0; w < FW; ++w) M = fmaxf(M, m_l[w][col]);
+    for (int u = 0; u < CT; ++u) {
+        const int have = cols - u * 16 < 16 ? cols - u * 16 : 16;          // (may be none)
+        if (u) __syncthreads();
+        l[u] += __shfl_xor(l[u], 16); l[u] += __shfl_xor(l[u], 32);
+        if (lr < have) {
 #pragma unroll
-        for (int w = 0; w < FW; ++w) { const float f = __builtin_amdgcn_exp2f(m_l[w][col] - M); v += acc_l[(w * 16 + col) * LD + d] * f; sum += l_l[w][col] * f; }
-        if (splits == 1) store(col, d, sum == 0.0f ? 0.0f : v / sum);
-        else {
-            float * r = part + (s * 16 + col) * (D + 2);
-            st_shared(r + d, v);
-            if (d == 0) { st_shared(r + D, M); st_shared(r + D + 1, sum); }
+            for (int t = 0; t < VT; ++t) *(f32x4 *) (acc_l + (wave * 16 + lr) * LD + t * 16 + lg * 4) = acc[u][t];
+            if (lg == 0) { m_l[wave][lr] = m[u]; l_l[wave][lr] = l[u]; }
+        }
+        __syncthreads();
+        for (int o = threadIdx.x; o < have * (D / 4); o += FW * 64) {
+            const int col = o / (D / 4), d = o % (D / 4) * 4;
+            float M = NONE, sum = 0.0f;
+            f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int w = 0; w < FW; ++w) M = fmaxf(M, m_l[w][col]);
+#pragma unroll
+            for (int w = 0; w < FW; ++w) { const float f = __builtin_amdgcn_exp2f(m_l[w][col] - M); v += *(const f32x4 *) (acc_l + (w * 16 + col) * LD + d) * f; sum += l_l[w][col] * f; }
+            if (splits == 1) store(u * 16 + col, d, v * (sum == 0.0f ? 0.0f : 1.0f / sum));
+            else {
+                put(part + (size_t) (s * COLS + u * 16 + col) * D + d, v);
+                if (d == 0) put(part + (size_t) splits * COLS * D + (s * COLS + u * 16 + col) * 2, M, sum);
+            }
         }
     }
-    if (splits == 1) return;
-    // partial sums out, then a ticket; the workgroup that draws the last one joins them in their order and leaves the ticket as it was
-    pm_vm_drain();
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        unsigned * tk = (unsigned *) a.work + slot;
-        is_last = __hip_atomic_fetch_add(tk, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned) splits - 1;
-        if (is_last) __hip_atomic_store(tk, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
-    __syncthreads();
-    if (!is_last) return;
-    for (int o = threadIdx.x; o < splits * 32; o += FW * 64) if ((o >> 1 & 15) < cols) ml[o] = ld_shared(part + (o >> 1) * (D + 2) + D + (o & 1));
-    __syncthreads();
-    for (int o = threadIdx.x; o < cols * D; o += FW * 64) {
-        const int col = o / D, d = o % D;
-        float M = NONE, v = 0.0f, sum = 0.0f;
-        for (int k = 0; k < splits; ++k) M = fmaxf(M, ml[(k * 16 + col) * 2]);
-        for (int k0 = 0; k0 < splits; k0 += 8) {
-            float r[8];
-#pragma unroll
-            for (int k = 0; k < 8; ++k) r[k] = ld_shared(part + ((k0 + k < splits ? k0 + k : splits - 1) * 16 + col) * (D + 2) + d);
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-                if (k0 + k < splits) { const float f = __builtin_amdgcn_exp2f(ml[((k0 + k) * 16 + col) * 2] - M); v += r[k] * f; sum += ml[((k0 + k) * 16 + col) * 2 + 1] * f; }
-        }
-        store(col, d, sum == 0.0f ? 0.0f : v / sum);
-    }
+    if (splits > 1 && last_of(a.work, slot, splits)) join<D, COLS>(part, splits, cols, acc_l, store);
 }
 
 // ---- prompts ----------------------------------------------------------------------------------------------------------------
 constexpr int TC = 128;                                    // columns of a tile: 32 per wave
 
-template <typename T, int NB, bool WIDE> __global__ __launch_bounds__(256) void tiles_kernel(pm_kv4_cache c, pm_kv4_attn a, int splits) {
+template <typename T, int NB, bool WIDE> __global__ __launch_bounds__(256, NB <= 4 ? 2 : 1) void tiles_kernel(pm_kv4_cache c, pm_kv4_attn a, int splits) {
     constexpr int D = NB * 32, KS = D / 16, VT = D / 32, KL = D * 2 + 16, VL = PM_PAGE * 2 + 16;      // LDS rows are an odd number of 16-byte pieces: no bank is asked twice
     typedef pm_kv4_slab<NB> S;
     extern __shared__ __attribute__((aligned(16))) char lds[];            // K [64][KL], V^T [D][VL]
     char * k_l = lds, * v_l = lds + PM_PAGE * KL;
     __shared__ uint8_t bad_l[16];
-    __shared__ int is_last;
     const int G = c.G, R = a.H / G, g = blockIdx.x % G, s = blockIdx.y;
     const int at = a.n_tiles - 1 - (int) (blockIdx.x / G);                // (later tiles see more keys: they start first)
     const size_t slot = blockIdx.x;
@@ -375,11 +456,14 @@ template <typename T, int NB, bool WIDE> __global__ __launch_bounds__(256) void 
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
                 const f16x2 sc = half_of(xks, b);
-                *(f16x8 *) (k_l + kr * KL + (b * 4 + kg) * 16) = eight(pair(xk[b], 0, sc), pair(xk[b], 1, sc), pair(xk[b], 2, sc), pair(xk[b], 3, sc));
+                f16x2 n[4];
+                codes(xk[b], n);
+                *(f16x8 *) (k_l + kr * KL + (b * 4 + kg) * 16) = eight(n[0] * sc, n[1] * sc, n[2] * sc, n[3] * sc);
+                codes(xv[b], n);
                 const f16x2 s0 = __builtin_bit_cast(f16x2, xvs[b][0]), s1 = __builtin_bit_cast(f16x2, xvs[b][1]);
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
-                    *(u32x2 *) (v_l + (b * 32 + h * 16 + vn) * VL + vq * 8) = u32x2{__builtin_bit_cast(uint32_t, pair(xv[b], h, s0)), __builtin_bit_cast(uint32_t, pair(xv[b], h + 2, s1))};
+                    *(u32x2 *) (v_l + (b * 32 + h * 16 + vn) * VL + vq * 8) = u32x2{__builtin_bit_cast(uint32_t, n[h] * s0), __builtin_bit_cast(uint32_t, n[h + 2] * s1)};
             }
             __syncthreads();
         }
@@ -446,72 +530,59 @@ template <typename T, int NB, bool WIDE> __global__ __launch_bounds__(256) void 
 #pragma unroll
         for (int t = 0; t < VT; ++t)
 #pragma unroll
-            for (int e = 0; e < 16; e += 4) {
-                const int d = t * 32 + 2 * e + 4 * hf;
-                if constexpr (sizeof(T) == 2) *(PM_G u16x4 *) (o + d) = u16x4{f2bf(acc[t][e] * f), f2bf(acc[t][e + 1] * f), f2bf(acc[t][e + 2] * f), f2bf(acc[t][e + 3] * f)};
-                else *(PM_G f32x4 *) (o + d) = f32x4{acc[t][e] * f, acc[t][e + 1] * f, acc[t][e + 2] * f, acc[t][e + 3] * f};
-            }
+            for (int e = 0; e < 16; e += 4) st_out(o + t * 32 + 2 * e + 4 * hf, f32x4{acc[t][e], acc[t][e + 1], acc[t][e + 2], acc[t][e + 3]} * f);
         return;
     }
     float * part = a.work + TICKETS + slot * splits * TC * (D + 2);
     if (col < cols) {
-        float * r = part + ((size_t) s * TC + col) * (D + 2);
+        float * r = part + ((size_t) s * TC + col) * D;
 #pragma unroll
         for (int t = 0; t < VT; ++t)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) st_shared(r + t * 32 + 8 * (e >> 2) + 4 * hf + (e & 3), acc[t][e]);
-        if (hf == 0) { st_shared(r + D, m); st_shared(r + D + 1, l); }
+            for (int e = 0; e < 16; e += 4) put(r + t * 32 + 2 * e + 4 * hf, f32x4{acc[t][e], acc[t][e + 1], acc[t][e + 2], acc[t][e + 3]});
+        if (hf == 0) put(part + (size_t) splits * TC * D + (s * TC + col) * 2, m, l);
     }
-    pm_vm_drain();
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        unsigned * tk = (unsigned *) a.work + slot;
-        is_last = __hip_atomic_fetch_add(tk, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned) splits - 1;
-        if (is_last) __hip_atomic_store(tk, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
-    __syncthreads();
-    if (!is_last) return;
-    for (int o = threadIdx.x; o < cols * D; o += 256) {
-        const int k = o / D, d = o % D, to = row0 + k / R;
-        const float * r = part + (size_t) k * (D + 2);
-        float M = NONE, v = 0.0f, sum = 0.0f;
-        for (int z = 0; z < splits; ++z) M = fmaxf(M, ld_shared(r + (size_t) z * TC * (D + 2) + D));
-        for (int z = 0; z < splits; ++z) {
-            const float * q = r + (size_t) z * TC * (D + 2);
-            const float f = __builtin_amdgcn_exp2f(ld_shared(q + D) - M);
-            v += ld_shared(q + d) * f; sum += ld_shared(q + D + 1) * f;
-        }
-        if ((unsigned) to < (unsigned) a.n_tokens) ((T *) a.out)[(size_t) to * a.ldo + (g * R + k % R) * D + d] = from_f<T>(sum == 0.0f ? 0.0f : v / sum);
-    }
+    if (last_of(a.work, slot, splits))
+        join<D, TC>(part, splits, cols, (float *) lds, [&](int k, int d, f32x4 o) {
+            const int to = row0 + k / R;
+            if ((unsigned) to < (unsigned) a.n_tokens) st_out((T *) a.out + (size_t) to * a.ldo + (g * R + k % R) * D + d, o);
+        });
 }
 
+constexpr int FEW_WANT = 1024, FEW_LEAST = 4, FEW_MOST = 128, FEW_COLS = 48, TILES_WANT = 512, TILES_LEAST = 8, TILES_MOST = 32;
 // workgroups over which the keys of a slot are split: as many as fill the chip, none with less than `least` pages, and what the scratch holds
-int splits_of(const pm_kv4_attn & a, int64_t slots, int want, int least, int64_t floats) {
+int splits_of(const pm_kv4_attn & a, int64_t slots, int64_t busy, int want, int least, int most, int64_t floats) {
     const int64_t pages = ((int64_t) a.max_keys + PM_PAGE - 1) / PM_PAGE, room = a.work && a.work_floats > TICKETS ? (int64_t) (a.work_floats - TICKETS) / (slots * floats) : 1;
-    int64_t n = (want + slots - 1) / slots;
+    int64_t n = (want + busy - 1) / busy;
     n = n < pages / least ? n : pages / least;
     n = n < room ? n : room;
-    n = n < 64 ? n : 64;
+    n = n < most ? n : most;
     return slots > TICKETS || n < 1 ? 1 : (int) n;
 }
-constexpr int FEW_WANT = 1024, FEW_LEAST = 4, TILES_WANT = 512, TILES_LEAST = 8;
 
 template <typename T, int NB> int launch(const pm_kv4_cache & c, pm_kv4_attn a, hipStream_t st) {
     constexpr int D = NB * 32;
     constexpr bool WIDE = sizeof(T) == 4;
     const int R = a.H / c.G;
     if (a.window > 0) { const int64_t most = (int64_t) a.window + a.tile_tokens + 128 + a.first; if (most < a.max_keys) a.max_keys = (int) most; }
-    if (a.tile_tokens == 1 || R * a.tile_tokens <= 16) {
-        const int64_t slots = (int64_t) a.n_tiles * c.G * ((R + 15) / 16);
-        const size_t lds = (size_t) FW * 16 * (D + 4) * 4;
-        const int splits = splits_of(a, slots, FEW_WANT, FEW_LEAST, 16 * (D + 2));
-        pm_allow_big_lds((const void *) few_kernel<T, NB, WIDE>, lds);
-        hipLaunchKernelGGL((few_kernel<T, NB, WIDE>), dim3((unsigned) slots, splits), dim3(FW * 64), lds, st, c, a, splits);
+    // columns of a tile on the average: tile_tokens only bounds them
+    const int64_t cols = (int64_t) R * (a.n_tokens / a.n_tiles < a.tile_tokens ? (a.n_tokens + a.n_tiles - 1) / a.n_tiles : a.tile_tokens);
+    auto few = [&](auto kern, int ct) {
+        const int passes = (R * a.tile_tokens + 16 * ct - 1) / (16 * ct);
+        const int64_t slots = (int64_t) a.n_tiles * c.G * passes, busy = (int64_t) a.n_tiles * c.G * ((cols + 16 * ct - 1) / (16 * ct));
+        const int splits = splits_of(a, slots, busy, FEW_WANT, FEW_LEAST, FEW_MOST, 16 * ct * (D + 2));
+        const size_t acc = (size_t) FW * 16 * (D + 4) * 4, ml = (size_t) splits * 16 * ct * 8 + 4096, lds = acc > ml ? acc : ml;
+        pm_allow_big_lds((const void *) kern, lds);
+        hipLaunchKernelGGL(kern, dim3((unsigned) slots, splits), dim3(FW * 64), lds, st, c, a, passes, splits);
         return 0;
+    };
+    if (a.tile_tokens == 1 || cols <= FEW_COLS) {
+        if constexpr (NB <= (WIDE ? 3 : 4)) if (cols > 16) return few(few_kernel<T, NB, WIDE, 2>, 2);
+        return few(few_kernel<T, NB, WIDE, 1>, 1);
     }
     const int64_t slots = (int64_t) a.n_tiles * c.G;
-    const size_t lds = (size_t) PM_PAGE * (D * 2 + 16) + D * (PM_PAGE * 2 + 16);
-    const int splits = splits_of(a, slots, TILES_WANT, TILES_LEAST, TC * (D + 2));
+    const int splits = splits_of(a, slots, slots, TILES_WANT, TILES_LEAST, TILES_MOST, TC * (D + 2));
+    const size_t stage = (size_t) PM_PAGE * (D * 2 + 16) + D * (PM_PAGE * 2 + 16), ml = splits > 1 ? (size_t) splits * TC * 8 + 4096 : 0, lds = stage > ml ? stage : ml;
     pm_allow_big_lds((const void *) tiles_kernel<T, NB, WIDE>, lds);
     hipLaunchKernelGGL((tiles_kernel<T, NB, WIDE>), dim3((unsigned) slots, splits), dim3(256), lds, st, c, a, splits);
     return 0;

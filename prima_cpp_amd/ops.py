@@ -4,6 +4,8 @@ meaning; see include/prima_mi355.h for the reference function each one replaces)
 Tensors are torch CUDA tensors used purely as device memory handles; all compute happens in
 libprima_mi355.so on the current torch stream.
 """
+import struct
+
 import numpy as np
 import torch
 
@@ -625,15 +627,35 @@ class AttnKV4Args(L.C.Structure):
                 ("d_tiles", _vp), ("n_tiles", L.C.c_int32), ("tile_tokens", L.C.c_int32), ("max_keys", L.C.c_int32), ("n_tokens", L.C.c_int32), ("work", _vp), ("work_floats", _sz)]
 
 
-def _operands(*named):
-    """(name, tensor, dtypes, dimensions): what the kernels take for granted of tensors that they get as pointers - on the current device, rows whose values lie side by side"""
-    for name, t, dtypes, dims in named:
-        if t is None:
-            continue
-        if not isinstance(t, torch.Tensor) or t.device.type != "cuda" or t.device.index != torch.cuda.current_device():
-            raise L.PM355Error("%s: a tensor on the current HIP device is wanted" % name)
-        if t.dtype not in dtypes or t.dim() != dims or (t.numel() and t.stride(-1) != 1):
-            raise L.PM355Error("%s: %d dimensions of %s, the last one contiguous, are wanted" % (name, dims, " or ".join(str(d) for d in dtypes)))
+# the three structures in one call each (a decoded token's launch is a few microseconds: building ctypes structures field by field would take as long)
+_KV4_CACHE, _KV4_APPEND, _ATTN_KV4 = struct.Struct("@iiiPPii"), struct.Struct("@iiiPqPqiPPfPiifPP"), struct.Struct("@iiPqPqfiiPiiiiPN")
+_ACT = (torch.float32, torch.bfloat16)
+_ACT_TYPE = {torch.float32: F32, torch.bfloat16: L.BF16}
+_KV4_DIMS = (64, 96, 128, 192, 256)
+_kv4_calls = {}
+
+
+def _kv4_call(name, *args):
+    f = _kv4_calls.get(name)
+    if f is None:
+        f = _kv4_calls[name] = L.declare(name, _i32, {"pm355_kv4_load": [_vp, _vp, _vp, _i32, _vp, _vp, _vp], "pm355_pages_copy": [_vp, _sz, _sz, _i32, _i32, _vp, _i32, _vp]}.get(name, [_vp] * 3))
+    rc = f(*args)
+    if rc:
+        check(rc, name[6:])
+
+
+def _same_device(*tensors):
+    """the current device's index; an error where one of the tensors lies elsewhere"""
+    device = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and (not isinstance(t, torch.Tensor) or t.get_device() != device):
+            raise L.PM355Error("tensors on the current HIP device are wanted: got %s" % (t.device if isinstance(t, torch.Tensor) else type(t).__name__))
+    return device
+
+
+def _want(ok, what):
+    if not ok:
+        raise L.PM355Error(what)
 
 
 def kv4_page_bytes(n_head_kv, head_dim):
@@ -645,17 +667,24 @@ def kv4_page_bytes(n_head_kv, head_dim):
 
 
 def _kv4_cache(pages, table, n_head_kv, head_dim):
-    _operands(("pages", pages, (torch.uint8,), 2), ("table", table, (torch.int32,), 2))
-    if pages.shape[1] != kv4_page_bytes(n_head_kv, head_dim) or not pages.is_contiguous():
-        raise L.PM355Error("pages: contiguous [pages, %d] is wanted" % kv4_page_bytes(n_head_kv, head_dim))
-    if not table.numel() or not table.is_contiguous():
-        raise L.PM355Error("table: contiguous rows of page numbers, one per sequence, are wanted")
-    return KV4Cache(n_head_kv, head_dim, pages.shape[0], ptr(pages), ptr(table), table.shape[1], table.shape[0])
+    if head_dim not in _KV4_DIMS or n_head_kv < 1:
+        kv4_page_bytes(n_head_kv, head_dim)
+    size, (rows, cols) = n_head_kv * head_dim * 72, table.shape if table.dim() == 2 else (0, 0)
+    _want(pages.dtype is torch.uint8 and pages.dim() == 2 and pages.shape[1] == size and pages.is_contiguous(), "pages: contiguous uint8 [pages, %d] is wanted" % size)
+    _want(table.dtype is torch.int32 and rows and cols and table.is_contiguous(), "table: contiguous int32 rows of page numbers, one per sequence, are wanted")
+    return _KV4_CACHE.pack(n_head_kv, head_dim, pages.shape[0], pages.data_ptr(), table.data_ptr(), cols, rows)
 
 
-def _rows_of(name, t, n):
-    if t.shape[0] != n:
-        raise L.PM355Error("%s: %d rows are wanted, got %d" % (name, n, t.shape[0]))
+def _per_token(name, t, n):
+    _want(t.dtype is torch.int32 and t.dim() == 1 and t.shape[0] == n and (n < 2 or t.stride(0) == 1), "%s: %d contiguous int32 are wanted" % (name, n))
+    return t.data_ptr()
+
+
+def _rows(name, t, n, width, dtypes, unit):
+    """(pointer, values between rows) of [n, >= width] whose rows start at multiples of `unit` values"""
+    shape, (ld, one) = t.shape, t.stride() if t.dim() == 2 else (0, 0)
+    _want(len(shape) == 2 and shape[0] == n and shape[1] >= width and t.dtype in dtypes and one == 1, "%s: %d rows of %d contiguous values in %s are wanted" % (name, n, width, " or ".join(str(d) for d in dtypes)))
+    return t.data_ptr(), ld if n > 1 else width + -width % unit
 
 
 def rope_turns(n_dims, n_ctx_orig=8192, freq_base=10000.0, freq_scale=1.0, ext_factor=0.0, attn_factor=1.0, beta_fast=32.0, beta_slow=1.0, freq_factors=None):
@@ -673,43 +702,33 @@ def rope_turns(n_dims, n_ctx_orig=8192, freq_base=10000.0, freq_scale=1.0, ext_f
 def kv4_append(proj, pages, table, pos, seq, n_head, n_head_kv, head_dim, q=None, norm=False, norm_q=None, norm_k=None, eps=1e-6, turns=None, mscale=1.0, neox=False):
     """Queries normed and rotated (returned, [T, n_head * head_dim] in the type of proj), keys likewise and values into 4-bit pages. proj [T, >= (n_head + 2 n_head_kv) * head_dim] rows
     q | k | v, f32 or bf16; pages uint8 [n, kv4_page_bytes()], table int32 [sequences, pages of a sequence], pos, seq int32 [T]; turns (rope_turns): None rotates nothing."""
+    device = _same_device(proj, pages, table, pos, seq, q, norm_q, norm_k, turns)
     c = _kv4_cache(pages, table, n_head_kv, head_dim)
-    _operands(("proj", proj, (torch.float32, torch.bfloat16), 2), ("pos", pos, (torch.int32,), 1), ("seq", seq, (torch.int32,), 1), ("norm_q", norm_q, (torch.float32,), 1),
-              ("norm_k", norm_k, (torch.float32,), 1), ("turns", turns, (torch.float64,), 1))
-    T = proj.shape[0]
+    T, dtype = proj.shape[0], proj.dtype
+    at, ld = _rows("proj", proj, T, (n_head + 2 * n_head_kv) * head_dim, _ACT, 4)
     if q is None:
-        q = torch.empty(T, n_head * head_dim, dtype=proj.dtype, device=proj.device)
-    _operands(("q", q, (proj.dtype,), 2))
-    for name, t in (("pos", pos), ("seq", seq), ("q", q)):
-        _rows_of(name, t, T)
-    for name, t in (("norm_q", norm_q), ("norm_k", norm_k)):
-        if t is not None:
-            _rows_of(name, t, head_dim)
-            if not norm:
-                raise L.PM355Error("%s without norm=True" % name)
-    if proj.shape[1] < (n_head + 2 * n_head_kv) * head_dim or q.shape[1] < n_head * head_dim:
-        raise L.PM355Error("proj, q: rows of %d and %d values are wanted" % ((n_head + 2 * n_head_kv) * head_dim, n_head * head_dim))
-    if not T:
-        return q
-    ld = lambda t: t.stride(0) if t.shape[0] > 1 else t.shape[1] // 8 * 8  # noqa: E731
-    a = KV4AppendArgs(pm_type(proj), n_head, T, ptr(proj), ld(proj), ptr(q), ld(q), int(norm), ptr(norm_q), ptr(norm_k), float(eps), ptr(turns), 0 if turns is None else 2 * turns.numel(), int(neox),
-                      float(mscale), ptr(pos), ptr(seq))
-    f = L.declare("pm355_kv4_append", _i32, [L.C.POINTER(KV4Cache), L.C.POINTER(KV4AppendArgs), _vp])
-    check(f(L.C.byref(c), L.C.byref(a), stream_ptr()), "kv4_append")
+        q = torch.empty(T, n_head * head_dim, dtype=dtype, device=proj.device)
+    q_at, ldq = _rows("q", q, T, n_head * head_dim, (dtype,), 4)
+    for w in (norm_q, norm_k):
+        _want(w is None or (norm and w.dtype is torch.float32 and w.dim() == 1 and w.shape[0] == head_dim and w.stride(0) == 1), "norm weights: norm=True and %d contiguous float32 are wanted" % head_dim)
+    _want(turns is None or (turns.dtype is torch.float64 and turns.dim() == 1 and turns.is_contiguous()), "turns: contiguous float64 (rope_turns) is wanted")
+    pos, seq = _per_token("pos", pos, T), _per_token("seq", seq, T)
+    if T:
+        _kv4_call("pm355_kv4_append", c, _KV4_APPEND.pack(_ACT_TYPE[dtype], n_head, T, at, ld, q_at, ldq, norm, ptr(norm_q) or 0, ptr(norm_k) or 0, eps, ptr(turns) or 0,
+                                                          0 if turns is None else 2 * turns.shape[0], neox, mscale, pos, seq), torch._C._cuda_getCurrentRawStream(device))
     return q
 
 
 def kv4_load(pages, table, pos, seq, n_head_kv, head_dim):
     """(k, v): what the pages hold for these (sequence, position), f16 [T, n_head_kv, head_dim]"""
-    c = _kv4_cache(pages, table, n_head_kv, head_dim)
-    _operands(("pos", pos, (torch.int32,), 1), ("seq", seq, (torch.int32,), 1))
-    T = pos.shape[0]
-    _rows_of("seq", seq, T)
-    k, v = (torch.empty(T, n_head_kv, head_dim, dtype=torch.float16, device=pages.device) for _ in range(2))
+    device = _same_device(pages, table, pos, seq)
+    c, T = _kv4_cache(pages, table, n_head_kv, head_dim), pos.shape[0]
+    pos, seq = _per_token("pos", pos, T), _per_token("seq", seq, T)
+    kv = torch.empty(2, T, n_head_kv, head_dim, dtype=torch.float16, device=pages.device)
     if T:
-        f = L.declare("pm355_kv4_load", _i32, [L.C.POINTER(KV4Cache), _vp, _vp, _i32, _vp, _vp, _vp])
-        check(f(L.C.byref(c), ptr(pos), ptr(seq), T, ptr(k), ptr(v), stream_ptr()), "kv4_load")
-    return k, v
+        at = kv.data_ptr()
+        _kv4_call("pm355_kv4_load", c, pos, seq, T, at, at + T * n_head_kv * head_dim * 2, torch._C._cuda_getCurrentRawStream(device))
+    return kv.unbind()
 
 
 def kv4_tiles(entries, n_head, n_head_kv):
@@ -732,35 +751,30 @@ def kv4_work(n_head, n_head_kv, head_dim):
 def attn_kv4(q, pages, table, tiles, tile_tokens, max_keys, n_head, n_head_kv, head_dim, scale, window=0, n_first=0, out=None, work=None):
     """Attention of q [T, n_head * head_dim] (f32 or bf16) over 4-bit pages: causal, with window > 0 only the last `window` keys and the first n_first. tiles int32 [n, 4] {row, tokens,
     position, sequence} (kv4_tiles). Returns out, of which the rows that tiles name are written. work: kv4_work(), for one call at a time."""
+    device = _same_device(q, pages, table, tiles, out, work)
     c = _kv4_cache(pages, table, n_head_kv, head_dim)
-    _operands(("q", q, (torch.float32, torch.bfloat16), 2), ("tiles", tiles, (torch.int32,), 2), ("work", work, (torch.float32,), 1))
-    if q.shape[1] < n_head * head_dim or tiles.shape[1] != 4 or not tiles.is_contiguous():
-        raise L.PM355Error("q, tiles: rows of %d values and contiguous rows of 4 are wanted" % (n_head * head_dim))
+    T, n = q.shape[0], tiles.shape[0]
+    q_at, ldq = _rows("q", q, T, n_head * head_dim, _ACT, 8)
+    _want(tiles.dtype is torch.int32 and tiles.dim() == 2 and tiles.shape[1] == 4 and tiles.is_contiguous(), "tiles: contiguous int32 rows of 4 are wanted")
+    _want(work is None or (work.dtype is torch.float32 and work.is_contiguous()), "work: contiguous float32 is wanted")
     if out is None:
-        out = torch.empty(q.shape[0], n_head * head_dim, dtype=q.dtype, device=q.device)
-    _operands(("out", out, (q.dtype,), 2))
-    _rows_of("out", out, q.shape[0])
-    if out.shape[1] < n_head * head_dim:
-        raise L.PM355Error("out: rows of %d values are wanted" % (n_head * head_dim))
-    if not q.shape[0] or not tiles.shape[0]:
-        return out
-    ld = lambda t: t.stride(0) if t.shape[0] > 1 else t.shape[1] // 8 * 8  # noqa: E731
-    a = AttnKV4Args(pm_type(q), n_head, ptr(q), ld(q), ptr(out), ld(out), float(scale), window, n_first, ptr(tiles), tiles.shape[0], tile_tokens, max_keys, q.shape[0], ptr(work),
-                    0 if work is None else work.numel())
-    f = L.declare("pm355_attn_kv4", _i32, [L.C.POINTER(KV4Cache), L.C.POINTER(AttnKV4Args), _vp])
-    check(f(L.C.byref(c), L.C.byref(a), stream_ptr()), "attn_kv4")
+        out = torch.empty(T, n_head * head_dim, dtype=q.dtype, device=q.device)
+    out_at, ldo = _rows("out", out, T, n_head * head_dim, (q.dtype,), 8)
+    if T and n:
+        _kv4_call("pm355_attn_kv4", c, _ATTN_KV4.pack(_ACT_TYPE[q.dtype], n_head, q_at, ldq, out_at, ldo, scale, window, n_first, tiles.data_ptr(), n, tile_tokens, max_keys, T,
+                                                      0 if work is None else work.data_ptr(), 0 if work is None else work.numel()), torch._C._cuda_getCurrentRawStream(device))
     return out
 
 
 def pages_copy(pages, pairs):
     """pages[.., to] = pages[.., from] for (from, to) pairs on the host: uint8 [layers, n, page bytes] or [n, page bytes]; every `to` stands once and is no `from`"""
-    if pages.dim() == 2:
-        pages = pages[None]
-    _operands(("pages", pages, (torch.uint8,), 3))
-    if not pages[0].is_contiguous():
-        raise L.PM355Error("pages: contiguous layers are wanted")
-    pairs = np.ascontiguousarray(pairs, np.int32).reshape(-1, 2)
-    if not len(pairs):
-        return
-    f = L.declare("pm355_pages_copy", _i32, [_vp, _sz, _sz, _i32, _i32, _vp, _i32, _vp])
-    check(f(ptr(pages), pages.shape[2], pages.stride(0) if pages.shape[0] > 1 else pages[0].numel(), pages.shape[0], pages.shape[1], pairs.ctypes.data, len(pairs), stream_ptr()), "pages_copy")
+    device = _same_device(pages)
+    pairs = np.ascontiguousarray(pairs, np.int32)
+    shape, stride = pages.shape, pages.stride()
+    if len(shape) == 2:
+        shape, stride = (1, *shape), (0, *stride)
+    _want(len(shape) == 3 and pages.dtype is torch.uint8 and stride[1:] == (shape[2], 1), "pages: uint8 layers of contiguous pages are wanted")
+    _want(pairs.size == 0 or (pairs.ndim == 2 and pairs.shape[1] == 2), "pairs: [n, 2] is wanted")
+    if len(pairs):
+        _kv4_call("pm355_pages_copy", pages.data_ptr(), shape[2], stride[0] if shape[0] > 1 else shape[1] * shape[2], shape[0], shape[1], pairs.ctypes.data, len(pairs),
+                  torch._C._cuda_getCurrentRawStream(device))

@@ -166,6 +166,10 @@ def test_rope_turns():
             ops._dev = ops_dev
 
 
+def test_structures():
+    assert (ops._KV4_CACHE.size, ops._KV4_APPEND.size, ops._ATTN_KV4.size) == tuple(C.sizeof(t) for t in (ops.KV4Cache, ops.KV4AppendArgs, ops.AttnKV4Args))
+
+
 def test_tiles():
     t, n, keys = ops.kv4_tiles([(3, 10, 1), (0, 70, 1)], 32, 8)
     assert n == 4 and keys == 71 and t.tolist() == [[0, 1, 10, 3], [1, 1, 70, 0]]
