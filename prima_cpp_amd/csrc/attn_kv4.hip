@@ -21,22 +21,22 @@ typedef uint16_t u16x4 __attribute__((ext_vector_type(4)));
 
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float NONE = -1e30f;                             // running maximum before the first visible key
-constexpr float HELD = 8.0f;                               // probabilities are held times 2^HELD
+constexpr float HELD = 8.0f, SLACK = 6.0f;                 // probabilities are held times 2^HELD; the running maximum may lag by SLACK (2^14 < 65504), sums are seldom rescaled
 constexpr int TICKETS = 65536;                             // words of the scratch in front of the partial sums
 
 // N words (N halves) that lie side by side, a multiple of 4 N (2 N) bytes into a slab
-template <int N> __device__ __forceinline__ void ld_words(const char * p, uint32_t * w) {
-    if constexpr (N == 1) w[0] = *(const PM_G uint32_t *) p;
-    else if constexpr (N == 2) { const u32x2 t = *(const PM_G u32x2 *) p; w[0] = t.x; w[1] = t.y; }
+template <int N> __device__ __forceinline__ void ld_words(const PM_G char * p, uint32_t * w) {
+    if constexpr (N == 2) { const u32x2 t = *(const PM_G u32x2 *) p; w[0] = t.x; w[1] = t.y; }
     else if constexpr (N == 3) { const u32x3 t = *(const PM_G u32x3 *) p; w[0] = t.x; w[1] = t.y; w[2] = t.z; }
     else if constexpr (N == 4) { const u32x4 t = *(const PM_G u32x4 *) p; w[0] = t.x; w[1] = t.y; w[2] = t.z; w[3] = t.w; }
     else { ld_words<N / 2>(p, w); ld_words<N / 2>(p + 2 * N, w + N / 2); }
 }
-template <int N> __device__ __forceinline__ void ld_halves(const char * p, uint32_t * w) {
+template <int N> __device__ __forceinline__ void ld_halves(const PM_G char * p, uint32_t * w) {
     if constexpr (N == 3) {
         const PM_G uint16_t * h = (const PM_G uint16_t *) p;
         w[0] = h[0] | (uint32_t) h[1] << 16; w[1] = h[2];
-    } else ld_words<N / 2>(p, w);
+    } else if constexpr (N == 2) w[0] = *(const PM_G uint32_t *) p;
+    else ld_words<N / 2>(p, w);
 }
 __device__ __forceinline__ f16x2 half_of(const uint32_t * w, int i) {      // value i of packed halves, twice
     const f16x2 t = __builtin_bit_cast(f16x2, w[i >> 1]);
@@ -85,15 +85,15 @@ __device__ __forceinline__ bool last_of(float * work, size_t slot, int splits) {
     return true;
 }
 // The last one joins the splits in their order (results do not depend on who that is): 4 dimensions of a column per thread, up to 16 splits on their way at once - a load that comes from
-// another XCD's store takes about a microsecond, and one at a time 128 splits took 40. lds: splits * COLS * 2 + 1024 floats
-template <int D, int COLS, typename F> __device__ __forceinline__ void join(const float * part, int splits, int cols, float * lds, F && store) {
+// another XCD's store takes about a microsecond, and one at a time 128 splits took 40. lds: splits * COLS * 2 + 4 NT floats
+template <int D, int COLS, int NT, typename F> __device__ __forceinline__ void join(const float * part, int splits, int cols, float * lds, F && store) {
     __shared__ float inv[COLS];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const float * ml = part + (size_t) splits * COLS * D;
-    for (int o = threadIdx.x; o < splits * COLS; o += 256)
+    for (int o = threadIdx.x; o < splits * COLS; o += NT)
         if (o % COLS < cols) { const f32x2 v = *(const PM_G f32x2 *) (ml + 2 * o); lds[2 * o] = v.x; lds[2 * o + 1] = v.y; }
     __syncthreads();
-    for (int col = wave; col < cols; col += 4) {           // maximum and sum of a column by a wave; the factors of its splits take the place of their maxima
+    for (int col = wave; col < cols; col += NT / 64) {           // maximum and sum of a column by a wave; the factors of its splits take the place of their maxima
         float M = NONE, L = 0.0f;
         for (int k = lane; k < splits; k += 64) M = fmaxf(M, lds[(k * COLS + col) * 2]);
         M = all_max(M);
@@ -102,9 +102,9 @@ template <int D, int COLS, typename F> __device__ __forceinline__ void join(cons
         if (lane == 0) inv[col] = L == 0.0f ? 0.0f : 1.0f / L;
     }
     __syncthreads();
-    const int items = cols * (D / 4), groups = items < 256 ? 256 / items : 1;
+    const int items = cols * (D / 4), groups = items < NT ? NT / items : 1;
     float * sums = lds + splits * COLS * 2;
-    for (int o = threadIdx.x; o < items * groups; o += 256) {
+    for (int o = threadIdx.x; o < items * groups; o += NT) {
         const int grp = o / items, it = o % items, col = it / (D / 4), d = it % (D / 4) * 4;
         const float * p = part + (size_t) col * D + d;
         f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -125,7 +125,7 @@ template <int D, int COLS, typename F> __device__ __forceinline__ void join(cons
     }
     if (groups == 1) return;
     __syncthreads();
-    for (int it = threadIdx.x; it < items; it += 256) {
+    for (int it = threadIdx.x; it < items; it += NT) {
         f32x4 v = *(const f32x4 *) (sums + it * 4);
         for (int k = 1; k < groups; ++k) v += *(const f32x4 *) (sums + (k * items + it) * 4);
         const int col = it / (D / 4);
@@ -177,18 +177,53 @@ __device__ __forceinline__ pm_seen seen_by(const pm_kv4_cache & c, const pm_kv4_
 __device__ __forceinline__ int page_at(const pm_seen & s, int i) { return i < s.front ? i : s.p0 + i - s.front; }
 
 // ---- few columns ------------------------------------------------------------------------------------------------------------
-constexpr int FW = 4;                                      // waves of a workgroup
-template <int NB> struct pm_chunk { uint32_t k[2][NB], ks[2][(NB + 1) / 2], v[2][NB], vs[NB][4]; };      // codes and scales of 32 keys as a lane wants them
+constexpr int FW = 8, STAGES = 2;                          // waves of a workgroup; steps of a wave whose codes have a place in LDS
+// 32 keys in LDS: key codes (rows of 16 NB bytes), value codes, key scales, value scales [NB][32]
+template <int NB> struct pm_step {
+    static constexpr int V = 512 * NB, KS = 1024 * NB, VS = 1088 * NB, BYTES = 1152 * NB;
+    static constexpr int WIDE_LOADS = (512 * NB + 1023) / 1024, NARROW_LOADS = (64 * NB + 255) / 256, LOADS = 2 * (WIDE_LOADS + NARROW_LOADS);
+};
+// LDS <- 64 x 16 (64 x 4) bytes like pm_dma16, for codes that are read once
+__device__ __forceinline__ void dma16(const void * base, uint32_t voff, uint32_t dst) {
+    unsigned keep;
+    dst = (uint32_t) __builtin_amdgcn_readfirstlane((int) dst);
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt\n\ts_mov_b32 m0, %0"
+                 : "=&s"(keep) : "v"(voff), "s"(uniform_ptr((char *) base)), "s"(dst) : "memory");
+}
+__device__ __forceinline__ void dma4(const void * base, uint32_t voff, uint32_t dst) {
+    unsigned keep;
+    dst = (uint32_t) __builtin_amdgcn_readfirstlane((int) dst);
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2 nt\n\ts_mov_b32 m0, %0"
+                 : "=&s"(keep) : "v"(voff), "s"(uniform_ptr((char *) base)), "s"(dst) : "memory");
+}
+template <int N> __device__ __forceinline__ void lds_words(const char * p, uint32_t * w) {
+    if constexpr (N == 1) w[0] = *(const uint32_t *) p;
+    else if constexpr (N == 2) { const u32x2 t = *(const u32x2 *) p; w[0] = t.x; w[1] = t.y; }
+    else if constexpr (N == 4) { const u32x4 t = *(const u32x4 *) p; w[0] = t.x; w[1] = t.y; w[2] = t.z; w[3] = t.w; }
+    else if constexpr (N == 3) { w[0] = ((const uint32_t *) p)[0]; w[1] = ((const uint32_t *) p)[1]; w[2] = ((const uint32_t *) p)[2]; }
+    else { lds_words<N / 2>(p, w); lds_words<N / 2>(p + 2 * N, w + N / 2); }
+}
+template <int NB> __device__ __forceinline__ void lds_halves(const char * p, uint32_t * w) {
+    if constexpr (NB == 3) { const uint16_t * h = (const uint16_t *) p; w[0] = h[0] | (uint32_t) h[1] << 16; w[1] = h[2]; }
+    else lds_words<NB / 2>(p, w);
+}
 
+// consecutive numbers for the workgroups of an XCD (workgroup i starts on XCD i mod 8)
+__device__ __forceinline__ uint32_t swizzled() {
+    const uint32_t n = gridDim.x, x = blockIdx.x & 7, q = n >> 3, r = n & 7;
+    return x * q + (x < r ? x : r) + (blockIdx.x >> 3);
+}
 // CT column tiles of 16 per workgroup share the keys' way from codes to f16; `passes` workgroups take the columns of a tile
-template <typename T, int NB, bool WIDE, int CT> __global__ __launch_bounds__(FW * 64, NB <= (WIDE ? 4 : 6) ? 2 : 1) void few_kernel(pm_kv4_cache c, pm_kv4_attn a, int passes, int splits) {
+template <typename T, int NB, bool WIDE, int CT> __global__ __launch_bounds__(FW * 64, NB * CT <= 4 && !WIDE ? 4 : 2) void few_kernel(pm_kv4_cache c, pm_kv4_attn a, int passes, int splits) {
     constexpr int D = NB * 32, VT = D / 16, LD = D + 4, COLS = 16 * CT;
     typedef pm_kv4_slab<NB> S;
-    extern __shared__ __attribute__((aligned(16))) float acc_l[];         // [FW][16][LD], then maximum and sum [splits][COLS][2]
+    typedef pm_step<NB> Q;
+    extern __shared__ __attribute__((aligned(16))) char lds[];            // [FW][STAGES] steps; then [FW][16][LD] sums; then what join() wants
+    float * acc_l = (float *) lds;
     __shared__ float m_l[FW][16], l_l[FW][16];
-    // (passes without columns are neighbours, not every n-th workgroup: those would leave whole XCDs idle)
-    const int G = c.G, R = a.H / G, g = blockIdx.x % G, at = blockIdx.x / G % a.n_tiles, pass = blockIdx.x / G / a.n_tiles, s = blockIdx.y;
-    const size_t slot = blockIdx.x;
+    const uint32_t id = swizzled();
+    const int G = c.G, R = a.H / G, g = id % G, pass = id / G % passes, s = id / G / passes % splits, at = id / G / passes / splits;
+    const size_t slot = ((size_t) at * passes + pass) * G + g;
     const int32_t * tile = uniform_const_ptr(a.tiles) + (size_t) at * 4;
     const int row0 = tile[0], seq = tile[3], pos0 = tile[2] < 0x7fffff00 ? tile[2] : 0x7fffff00, n = tile[1] < a.tile_tokens ? tile[1] : a.tile_tokens;
     const int col0 = pass * COLS, left = n * R - col0, cols = left < COLS ? left : COLS;
@@ -202,24 +237,30 @@ template <typename T, int NB, bool WIDE, int CT> __global__ __launch_bounds__(FW
     const char * head = c.pages + (size_t) g * S::BYTES;
     auto page_of = [&](int i) __attribute__((always_inline)) { if (!known || i >= end) return -1; const int p = table[page_at(see, i >> 1)]; return (unsigned) p < (unsigned) c.n_pages ? p : -1; };
     const uint32_t krow = 8 * (lr >> 2) + (lr & 3);        // key of score row lr in the first 16 of a step (the second: + 4)
-    const uint32_t at_k = krow * 16 * NB + lg * 4 * NB, at_ks = krow * 2 * NB, at_v = lg * 128 * NB + lr * 4 * NB, at_vs = lg * 16;
-    // (no branch around the loads: behind one the compiler waits for everything that may be on its way. What is not there is read from page 0 and left alone)
-    auto load = [&](pm_chunk<NB> & x, int i, int page) __attribute__((always_inline)) {
-        const char * slab = uniform_ptr((char *) head + (size_t) (page < 0 ? 0 : page) * G * S::BYTES);
-        const int key = (i & 1) * 32;
-        const char * k = slab + S::K + key * 16 * NB, * ks = slab + S::KS + key * 2 * NB, * v = slab + S::V + key * 16 * NB, * vs = slab + S::VS + key * 2;
+    // Codes go from memory to LDS in whole lines and from there to the lanes that want them: straight to registers a quarter of a wave's lanes would each want 16 bytes of another line of 64,
+    // four times the lines a load can ask for per cycle. Rows whose pieces would meet in a bank are turned against each other.
+    constexpr int TURN = NB % 4 ? 0 : NB / 4;
+    char * const ring = lds + wave * STAGES * Q::BYTES;
+    const uint32_t ring_at = (uint32_t) (uintptr_t) (__attribute__((address_space(3))) char *) lds + wave * STAGES * Q::BYTES;
+    const uint32_t at_k = krow * 16 * NB + (TURN ? (lg ^ (krow >> 3 & 3)) : lg) * 4 * NB;
+    auto load = [&](int i, int page, int stage) __attribute__((always_inline)) {
+        const char * slab = uniform_ptr((char *) head + (size_t) (page < 0 ? 0 : page) * G * S::BYTES);      // (what is not there is read from page 0 and left alone)
+        const char * k = slab + S::K + (i & 1) * 512 * NB, * v = slab + S::V + (i & 1) * 512 * NB, * ks = slab + S::KS + (i & 1) * 64 * NB, * vs = slab + S::VS + (i & 1) * 64;
+        const uint32_t to = ring_at + stage * Q::BYTES;
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-            ld_words<NB>(k + at_k + b * 64 * NB, x.k[b]);
-            ld_words<NB>(v + at_v + b * 64 * NB, x.v[b]);
-            ld_halves<NB>(ks + at_ks + b * 8 * NB, x.ks[b]);
+        for (int j = 0; j < Q::WIDE_LOADS; ++j) {
+            const uint32_t o = lane * 16 + j * 1024, row = o / (16 * NB);
+            if (o < 512 * NB) { dma16(k, TURN ? o ^ (row >> 3 & 3) * (16 * TURN) : o, to + j * 1024); dma16(v, o, to + Q::V + j * 1024); }
         }
 #pragma unroll
-        for (int w = 0; w < NB; ++w) ld_words<4>(vs + at_vs + w * PM_PAGE * 2, x.vs[w]);
+        for (int j = 0; j < Q::NARROW_LOADS; ++j) {
+            const uint32_t o = lane * 4 + j * 256;
+            if (o < 64 * NB) { dma4(ks, o, to + Q::KS + j * 256); dma4(vs, (o >> 6) * (PM_PAGE * 2) + (o & 63), to + Q::VS + j * 256); }
+        }
     };
-    int i = 2 * s * per + wave, page = page_of(i), next = page_of(i + FW);
-    pm_chunk<NB> x0, x1;
-    load(x0, i, page);
+    int i = 2 * s * per + wave, page = page_of(i), next = page_of(i + FW), stage = 0;
+    if (i < end) load(i, page, 0);
+    if (i + FW < end) load(i + FW, next, 1);
 
     f16x8 qh[CT][NB], ql[WIDE ? CT : 1][NB];
     f32x4 acc[CT][VT];
@@ -253,16 +294,27 @@ template <typename T, int NB, bool WIDE, int CT> __global__ __launch_bounds__(FW
         for (int t = 0; t < VT; ++t) acc[u][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         m[u] = NONE; l[u] = 0.0f;
     }
-    auto step = [&](pm_chunk<NB> & x, int i) __attribute__((always_inline)) {
+    for (; i < end; i += FW) {
+        const int after = page_of(i + 2 * FW);
+        if (i + FW < end) asm volatile("s_waitcnt vmcnt(%0)" :: "n"(Q::LOADS) : "memory");      // (a wave's loads come back in their order)
+        else pm_vm_drain();
+        const char * x = ring + stage * Q::BYTES;
         const int k0 = page_at(see, i >> 1) * PM_PAGE + (i & 1) * 32, key0 = k0 + lg * 8;      // the lane's eight keys
         f32x4 s0[CT], s1[CT];
 #pragma unroll
         for (int u = 0; u < CT; ++u) s0[u] = s1[u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        uint32_t xk[2][NB], xs[2][(NB + 1) / 2], xv[2][NB], vs[NB][4];
+#pragma unroll
+        for (int b = 0; b < 2; ++b) { lds_words<NB>(x + at_k + b * 64 * NB, xk[b]); lds_halves<NB>(x + Q::KS + (krow + 4 * b) * 2 * NB, xs[b]); }
+#pragma unroll
+        for (int b = 0; b < 2; ++b) lds_words<NB>(x + Q::V + (2 * lg + b) * 64 * NB + lr * 4 * NB, xv[b]);
+#pragma unroll
+        for (int w = 0; w < NB; ++w) lds_words<4>(x + Q::VS + w * 64 + lg * 16, vs[w]);
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-            const f16x2 sa = half_of(x.ks[0], b), sb = half_of(x.ks[1], b);
+            const f16x2 sa = half_of(xs[0], b), sb = half_of(xs[1], b);
             f16x2 na[4], nb[4];
-            codes(x.k[0][b], na); codes(x.k[1][b], nb);
+            codes(xk[0][b], na); codes(xk[1][b], nb);
             const f16x8 ka = eight(na[0] * sa, na[1] * sa, na[2] * sa, na[3] * sa), kb = eight(nb[0] * sb, nb[1] * sb, nb[2] * sb, nb[3] * sb);
 #pragma unroll
             for (int u = 0; u < CT; ++u) {
@@ -272,13 +324,15 @@ template <typename T, int NB, bool WIDE, int CT> __global__ __launch_bounds__(FW
             }
         }
         // a step that not every column sees whole: hidden keys count nothing, whatever their slots hold
-        const bool whole = k0 + 31 <= see.lo && !(a.window > 0 && k0 <= see.hi - a.window);
+        const bool whole = page >= 0 && k0 + 31 <= see.lo && !(a.window > 0 && k0 <= see.hi - a.window);
         uint32_t bad = 0;
-        if (!whole)
+        if (!whole) {
+            asm volatile("");                              // (a branch: as selects this would cost every step as much as the products' operands)
 #pragma unroll
             for (int w = 0; w < NB; ++w)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) bad |= finite(x.vs[w][j]) << 2 * j;
+                for (int j = 0; j < 4; ++j) bad |= finite(vs[w][j]) << 2 * j;
+        }
         f16x8 ph[CT], pl[CT];
 #pragma unroll
         for (int u = 0; u < CT; ++u) {
@@ -286,11 +340,12 @@ template <typename T, int NB, bool WIDE, int CT> __global__ __launch_bounds__(FW
 #pragma unroll
             for (int j = 0; j < 8; ++j) f[j] = j < 4 ? s0[u][j & 3] : s1[u][j & 3];
             if (!whole) {
-                const int low = a.window > 0 ? pos[u] - a.window + 1 : 0;
+                asm volatile("");
+                const int last = page < 0 ? -1 : pos[u], low = a.window > 0 ? pos[u] - a.window + 1 : 0;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     const int key = key0 + j;
-                    const bool ok = key <= pos[u] && (key >= low || key < a.first);
+                    const bool ok = key <= last && (key >= low || key < a.first);
                     f[j] = ok ? (bad >> j & 1 ? NAN : f[j]) : -INFINITY;
                 }
             }
@@ -299,7 +354,7 @@ template <typename T, int NB, bool WIDE, int CT> __global__ __launch_bounds__(FW
             for (int j = 1; j < 8; ++j) mx = fmaxf(mx, f[j]);
             mx = fmaxf(mx, __shfl_xor(mx, 16)); mx = fmaxf(mx, __shfl_xor(mx, 32));
             mx = fmaxf(mx * cf[u], NONE);
-            if (__any(mx > m[u])) {
+            if (__any(mx > m[u] + SLACK)) {
                 const float mn = fmaxf(m[u], mx), corr = __builtin_amdgcn_exp2f(m[u] - mn);
                 m[u] = mn; l[u] *= corr;
 #pragma unroll
@@ -316,8 +371,8 @@ template <typename T, int NB, bool WIDE, int CT> __global__ __launch_bounds__(FW
         for (int w = 0; w < NB; ++w) {
             f16x2 sc[4], na[4], nb[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) sc[j] = __builtin_bit_cast(f16x2, x.vs[w][j]);
-            codes(x.v[0][w], na); codes(x.v[1][w], nb);
+            for (int j = 0; j < 4; ++j) sc[j] = __builtin_bit_cast(f16x2, vs[w][j]);
+            codes(xv[0][w], na); codes(xv[1][w], nb);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const f16x8 v = eight(na[h] * sc[0], na[h + 2] * sc[1], nb[h] * sc[2], nb[h + 2] * sc[3]);
@@ -328,16 +383,11 @@ template <typename T, int NB, bool WIDE, int CT> __global__ __launch_bounds__(FW
                 }
             }
         }
-    };
-    // the next 32 keys are on their way while these are worked on, and the page after them is looked up
-    for (; i < end; i += 2 * FW) {
-        const int after = page_of(i + 2 * FW), then = page_of(i + 3 * FW);
-        load(x1, i + FW, next);
-        if (page >= 0) step(x0, i);
-        load(x0, i + 2 * FW, after);
-        if (next >= 0) step(x1, i + FW);
-        page = after; next = then;
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (the stage is read: it may be written)
+        if (i + 2 * FW < end) load(i + 2 * FW, after, stage);
+        page = next; next = after; stage ^= 1;
     }
+    __syncthreads();                                       // (the rings' LDS is the sums')
     auto store = [&](int col, int d, f32x4 o) {
         const int row = row0 + (col0 + col) / R;
         if ((unsigned) row < (unsigned) a.n_tokens) st_out((T *) a.out + (size_t) row * a.ldo + (g * R + (col0 + col) % R) * D + d, o);
@@ -369,7 +419,7 @@ template <typename T, int NB, bool WIDE, int CT> __global__ __launch_bounds__(FW
             }
         }
     }
-    if (splits > 1 && last_of(a.work, slot, splits)) join<D, COLS>(part, splits, cols, acc_l, store);
+    if (splits > 1 && last_of(a.work, slot, splits)) join<D, COLS, FW * 64>(part, splits, cols, acc_l, store);
 }
 
 // ---- prompts ----------------------------------------------------------------------------------------------------------------
@@ -404,7 +454,7 @@ template <typename T, int NB, bool WIDE> __global__ __launch_bounds__(256, NB <=
     uint32_t xk[NB], xks[(NB + 1) / 2], xv[NB], xvs[NB][2];
     auto load = [&](int page) __attribute__((always_inline)) {
         if (page < 0) return;
-        const char * slab = head + (size_t) page * G * S::BYTES;
+        const PM_G char * slab = (const PM_G char *) uniform_ptr((char *) head + (size_t) page * G * S::BYTES);
         ld_words<NB>(slab + S::K + kr * 16 * NB + kg * 4 * NB, xk);
         ld_halves<NB>(slab + S::KS + kr * 2 * NB, xks);
         ld_words<NB>(slab + S::V + vq * 64 * NB + vn * 4 * NB, xv);
@@ -498,7 +548,7 @@ template <typename T, int NB, bool WIDE> __global__ __launch_bounds__(256, NB <=
 #pragma unroll
             for (int e = 0; e < 16; ++e) mx = fmaxf(mx, sc[t][e]);
         mx = fmaxf(fmaxf(mx, __shfl_xor(mx, 32)) * cf, NONE);
-        if (__any(mx > m)) {
+        if (__any(mx > m + SLACK)) {
             const float mn = fmaxf(m, mx), corr = __builtin_amdgcn_exp2f(m - mn);
             m = mn; l *= corr;
 #pragma unroll
@@ -543,13 +593,13 @@ template <typename T, int NB, bool WIDE> __global__ __launch_bounds__(256, NB <=
         if (hf == 0) put(part + (size_t) splits * TC * D + (s * TC + col) * 2, m, l);
     }
     if (last_of(a.work, slot, splits))
-        join<D, TC>(part, splits, cols, (float *) lds, [&](int k, int d, f32x4 o) {
+        join<D, TC, 256>(part, splits, cols, (float *) lds, [&](int k, int d, f32x4 o) {
             const int to = row0 + k / R;
             if ((unsigned) to < (unsigned) a.n_tokens) st_out((T *) a.out + (size_t) to * a.ldo + (g * R + k % R) * D + d, o);
         });
 }
 
-constexpr int FEW_WANT = 1024, FEW_LEAST = 4, FEW_MOST = 128, FEW_COLS = 48, TILES_WANT = 512, TILES_LEAST = 8, TILES_MOST = 32;
+constexpr int FEW_WANT = 256, FEW_LEAST = 4, FEW_MOST = 128, FEW_COLS = 48, TILES_WANT = 512, TILES_LEAST = 8, TILES_MOST = 32;
 // workgroups over which the keys of a slot are split: as many as fill the chip, none with less than `least` pages, and what the scratch holds
 int splits_of(const pm_kv4_attn & a, int64_t slots, int64_t busy, int want, int least, int most, int64_t floats) {
     const int64_t pages = ((int64_t) a.max_keys + PM_PAGE - 1) / PM_PAGE, room = a.work && a.work_floats > TICKETS ? (int64_t) (a.work_floats - TICKETS) / (slots * floats) : 1;
@@ -571,9 +621,10 @@ template <typename T, int NB> int launch(const pm_kv4_cache & c, pm_kv4_attn a, 
         const int passes = (R * a.tile_tokens + 16 * ct - 1) / (16 * ct);
         const int64_t slots = (int64_t) a.n_tiles * c.G * passes, busy = (int64_t) a.n_tiles * c.G * ((cols + 16 * ct - 1) / (16 * ct));
         const int splits = splits_of(a, slots, busy, FEW_WANT, FEW_LEAST, FEW_MOST, 16 * ct * (D + 2));
-        const size_t acc = (size_t) FW * 16 * (D + 4) * 4, ml = (size_t) splits * 16 * ct * 8 + 4096, lds = acc > ml ? acc : ml;
+        const size_t ring = (size_t) FW * STAGES * pm_step<NB>::BYTES, acc = (size_t) FW * 16 * (D + 4) * 4, ml = splits > 1 ? (size_t) splits * 16 * ct * 8 + FW * 64 * 16 : 0;
+        const size_t lds = ring > acc ? (ring > ml ? ring : ml) : acc > ml ? acc : ml;
         pm_allow_big_lds((const void *) kern, lds);
-        hipLaunchKernelGGL(kern, dim3((unsigned) slots, splits), dim3(FW * 64), lds, st, c, a, passes, splits);
+        hipLaunchKernelGGL(kern, dim3((unsigned) (slots * splits)), dim3(FW * 64), lds, st, c, a, passes, splits);
         return 0;
     };
     if (a.tile_tokens == 1 || cols <= FEW_COLS) {

@@ -14,25 +14,41 @@ typedef uint16_t u16x4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ void st4(float * p, const float * v) { *(PM_G f32x4 *) p = f32x4{v[0], v[1], v[2], v[3]}; }
 __device__ __forceinline__ void st4(uint16_t * p, const float * v) { *(PM_G u16x4 *) p = u16x4{f2bf(v[0]), f2bf(v[1]), f2bf(v[2]), f2bf(v[3])}; }
 
+// what the other lanes of a group of 2, 4, 8, 16, 32 hold, once the smaller groups agree: DPP within rows of 16, a lane swap between them
+template <int M> __device__ __forceinline__ uint32_t other(uint32_t v) {
+    if constexpr (M == 16) return other_row(v);
+    else return (uint32_t) __builtin_amdgcn_update_dpp(0, (int) v, M == 1 ? 0xB1 : M == 2 ? 0x4E : M == 4 ? 0x141 : 0x140, 0xF, 0xF, true);
+}
+template <int M> __device__ __forceinline__ float other(float v) { return __builtin_bit_cast(float, other<M>(__builtin_bit_cast(uint32_t, v))); }
+template <int M> __device__ __forceinline__ double other(double v) {
+    const u32x2 t = __builtin_bit_cast(u32x2, v);
+    return __builtin_bit_cast(double, u32x2{other<M>((uint32_t) t.x), other<M>((uint32_t) t.y)});
+}
 template <int LPH, typename F> __device__ __forceinline__ F head_sum(F v) {       // over the LPH lanes of a head row
-#pragma unroll
-    for (int m = 1; m < LPH; m *= 2) v += __shfl_xor(v, m);
+    v += other<1>(v); v += other<2>(v); v += other<4>(v);
+    if constexpr (LPH >= 16) v += other<8>(v);
+    if constexpr (LPH >= 32) v += other<16>(v);
     return v;
 }
 // scale (f16 bits) of a block whose 32 values lie in four neighbouring lanes, 8 each; NaN where the row holds a NaN or an infinity
-template <int LPH> __device__ __forceinline__ uint16_t block_scale(const float * x, bool on) {
-    float hi = -INFINITY, lo = INFINITY, bad = 0.0f;
+template <int LPH> __device__ __forceinline__ uint16_t block_scale(const float * x) {
+    float hi = x[0], lo = x[0], bad = 0.0f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) { hi = fmaxf(hi, x[j]); lo = fminf(lo, x[j]); bad += on ? x[j] * 0.0f : 0.0f; }       // (0 * NaN, 0 * inf: NaN)
-#pragma unroll
-    for (int m = 1; m < 4; m *= 2) { hi = fmaxf(hi, __shfl_xor(hi, m)); lo = fminf(lo, __shfl_xor(lo, m)); }
+    for (int j = 0; j < 8; ++j) { hi = fmaxf(hi, x[j]); lo = fminf(lo, x[j]); bad = fmaf(x[j], 0.0f, bad); }       // (0 * NaN, 0 * inf: NaN)
+    hi = fmaxf(hi, other<1>(hi)); lo = fminf(lo, other<1>(lo));
+    hi = fmaxf(hi, other<2>(hi)); lo = fminf(lo, other<2>(lo));
     bad = head_sum<LPH>(bad);
     const float s = fminf(fmaxf((hi >= -lo ? hi : lo) * -0.125f, -8188.0f), 8188.0f);
     return bad == 0.0f ? f2h(s) : (uint16_t) 0x7e00;
 }
-__device__ __forceinline__ uint32_t code_of(float x, float s) {
-    if (!(s != 0.0f) || !(s == s)) return 8;               // (an empty block, a row that is not finite)
-    return (uint32_t) (int) (fminf(fmaxf(rintf(x / s), -8.0f), 7.0f) + 8.0f);
+// codes 0 .. 15 of eight values. r = 1 / s to half a unit; x r, corrected by its remainder, is then x / s as rounded once, so that a tie between two codes is seen as one
+__device__ __forceinline__ void block_codes(const float * x, uint16_t scale, float * c) {
+    const float s = h2f(scale), r = s != 0.0f && s == s ? 1.0f / s : 0.0f;        // (an empty block, a row that is not finite)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const float q = x[j] * r;
+        c[j] = __builtin_amdgcn_fmed3f(rintf(fmaf(fmaf(-q, s, x[j]), r, q)), -8.0f, 7.0f) + 8.0f;
+    }
 }
 
 // values of a lane on their way: two groups of four
@@ -82,47 +98,20 @@ template <typename T, int NB> __global__ __launch_bounds__(256) void append_kern
         cs[j][1] = s * (double) a.mscale;
     }
     lds_done();
-    for (int n = part; n < N; n += parts) {
-        float x[8];
+    int n = part;
+    float x[8];
+    auto take = [&](int heads, int h) __attribute__((always_inline)) {       // this step's values, the next one's on their way; whether this lane has any
         widen(next, x);
         next = load(n + parts < N ? n + parts : n);
-        const bool key = n < NG, val = !key && n < 2 * NG;
-        const int h = (key ? n : val ? n - NG : n - 2 * NG) * RPW + sub;
-        const bool live = on && h < (key || val ? G : a.H);
-        if (!live)
+        const bool live = on && h < heads;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = 0.0f;
-        if (!key && !val) {
-            if (a.norm) {
-                float ss = 0.0f;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) ss = fmaf(x[j], x[j], ss);
-                const float r = 1.0f / sqrtf(head_sum<LPH>(ss) / (float) D + a.eps);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) x[j] *= r * (a.wq ? a.wq[(j < 4 ? o0 : o1 - 4) + j] : 1.0f);
-            }
-            if (turn)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    float & p = a.neox ? x[j] : x[2 * j], & q = a.neox ? x[j + 4] : x[2 * j + 1];
-                    const float k = (float) cs[i * 4 + j][0], s = (float) cs[i * 4 + j][1], u = p, v = q;
-                    p = u * k - v * s; q = v * k + u * s;
-                }
-            if (live) { T * d = (T *) a.q + (size_t) t * a.ldq + h * D; st4(d + o0, x); st4(d + o1, x + 4); }
-            continue;
-        }
-        char * slab = slab0 + (size_t) h * S::BYTES;
-        if (val) {
-            const uint16_t sb = block_scale<LPH>(x, live);
-            const float s = h2f(sb);
-            if (!live || page < 0) continue;
-            char * at_v = slab + S::V + (slot >> 2) * 64 * NB + (i >> 2) * 4 + pm_kv4_vbyte(slot);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) *(PM_G uint8_t *) (at_v + ((i & 3) * 4 + j) * 4 * NB) = (uint8_t) (code_of(x[j], s) | code_of(x[j + 4], s) << 4);
-            if ((i & 3) == 0) *(PM_G uint16_t *) (slab + S::VS + ((i >> 2) * PM_PAGE + slot) * 2) = sb;
-            continue;
-        }
-        // keys: 64 bits up to the one rounding to 32, so that a code never depends on the order of a sum
+        for (int j = 0; j < 8; ++j) x[j] = live ? x[j] : 0.0f;
+        return live;
+    };
+    // keys: 64 bits up to the one rounding to 32, so that a code never depends on the order of a sum
+    for (; n < NG; n += parts) {
+        const int h = n * RPW + sub;
+        const bool live = take(G, h);
         double y[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) y[j] = x[j];
@@ -143,21 +132,61 @@ template <typename T, int NB> __global__ __launch_bounds__(256) void append_kern
             }
         // into the order of the page: lane i holds dimensions 8 i .. 8 i + 7
         float * kb = keys_l[wave][sub];
-        if (live)
+        if (on)
 #pragma unroll
             for (int j = 0; j < 4; ++j) { kb[o0 + j] = (float) y[j]; kb[o1 + j] = (float) y[j + 4]; }
         lds_done();
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[j] = live ? kb[i * 8 + j] : 0.0f;
         lds_done();
-        const uint16_t sb = block_scale<LPH>(x, live);
+        const uint16_t sb = block_scale<LPH>(x);
+        float q[8];
+        block_codes(x, sb, q);
         if (!live || page < 0) continue;
-        const float s = h2f(sb);
-        uint32_t w = 0;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) w |= code_of(x[j], s) << ((j & 1) * 16 + (j >> 1) * 4);
-        *(PM_G uint32_t *) (slab + S::K + slot * 16 * NB + (i & 3) * 4 * NB + (i >> 2) * 4) = w;
+        char * slab = slab0 + (size_t) h * S::BYTES;
+        // dimensions 0, 2, 4, 6 are the nibbles of the low half, 1, 3, 5, 7 of the high one
+        const uint32_t lo = (uint32_t) fmaf(q[6], 4096.0f, fmaf(q[4], 256.0f, fmaf(q[2], 16.0f, q[0]))), hi = (uint32_t) fmaf(q[7], 4096.0f, fmaf(q[5], 256.0f, fmaf(q[3], 16.0f, q[1])));
+        *(PM_G uint32_t *) (slab + S::K + slot * 16 * NB + (i & 3) * 4 * NB + (i >> 2) * 4) = lo | hi << 16;
         if ((i & 3) == 0) *(PM_G uint16_t *) (slab + S::KS + (slot * NB + (i >> 2)) * 2) = sb;
+    }
+    for (; n < 2 * NG; n += parts) {
+        const int h = (n - NG) * RPW + sub;
+        const bool live = take(G, h);
+        const uint16_t sb = block_scale<LPH>(x);
+        float q[8];
+        block_codes(x, sb, q);
+        if (!live || page < 0) continue;
+        char * slab = slab0 + (size_t) h * S::BYTES, * at_v = slab + S::V + (slot >> 2) * 64 * NB + (i >> 2) * 4 + pm_kv4_vbyte(slot);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) *(PM_G uint8_t *) (at_v + ((i & 3) * 4 + j) * 4 * NB) = (uint8_t) (uint32_t) fmaf(q[j + 4], 16.0f, q[j]);
+        if ((i & 3) == 0) *(PM_G uint16_t *) (slab + S::VS + ((i >> 2) * PM_PAGE + slot) * 2) = sb;
+    }
+    if (n >= N) return;
+    float w[8], ck[4], sk[4];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w[j] = a.wq ? a.wq[(j < 4 ? o0 : o1 - 4) + j] : 1.0f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) { ck[j] = turn ? (float) cs[i * 4 + j][0] : 1.0f; sk[j] = turn ? (float) cs[i * 4 + j][1] : 0.0f; }
+    for (; n < N; n += parts) {
+        const int h = (n - 2 * NG) * RPW + sub;
+        const bool live = take(a.H, h);
+        if (a.norm) {
+            float ss = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) ss = fmaf(x[j], x[j], ss);
+            const float r = __builtin_amdgcn_rsqf(head_sum<LPH>(ss) * (1.0f / D) + a.eps);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] *= r * w[j];
+        }
+        if (rot) {
+            if (a.neox)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) { const float u = x[j], v = x[j + 4]; x[j] = u * ck[j] - v * sk[j]; x[j + 4] = v * ck[j] + u * sk[j]; }
+            else
+#pragma unroll
+                for (int j = 0; j < 4; ++j) { const float u = x[2 * j], v = x[2 * j + 1]; x[2 * j] = u * ck[j] - v * sk[j]; x[2 * j + 1] = v * ck[j] + u * sk[j]; }
+        }
+        if (live) { T * d = (T *) a.q + (size_t) t * a.ldq + h * D; st4(d + o0, x); st4(d + o1, x + 4); }
     }
 }
 
@@ -194,8 +223,8 @@ template <int NB> __global__ __launch_bounds__(256) void load_kernel(pm_kv4_cach
 #define PM_KV4_DIMS(CALL) switch (c.d) { case 64: CALL(2); break; case 96: CALL(3); break; case 128: CALL(4); break; case 192: CALL(6); break; case 256: CALL(8); break; default: return PM355_E_UNSUPPORTED; }
 
 int pm_launch_kv4_append(const pm_kv4_cache & c, const pm_kv4_append & a, hipStream_t st) {
-    // waves per token: one where tokens alone give every SIMD two, down to one per group of head rows
-    const int rpw = c.d <= 64 ? 8 : c.d <= 128 ? 4 : 2, groups = 2 * ((c.G + rpw - 1) / rpw) + (a.H + rpw - 1) / rpw, fill = 2048 / a.T;
+    // waves per token: one where tokens alone give every SIMD eight, down to one per group of head rows
+    const int rpw = c.d <= 64 ? 8 : c.d <= 128 ? 4 : 2, groups = 2 * ((c.G + rpw - 1) / rpw) + (a.H + rpw - 1) / rpw, fill = 8192 / a.T;
     const int parts = fill < 1 ? 1 : fill < groups ? fill : groups;
     const int64_t blocks = ((int64_t) a.T * parts + 3) / 4;
     if (blocks > 0x3fffffff) return PM355_E_SHAPE;
