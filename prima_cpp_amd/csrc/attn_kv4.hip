@@ -42,20 +42,21 @@ __device__ __forceinline__ f16x2 half_of(const uint32_t * w, int i) {      // va
     const f16x2 t = __builtin_bit_cast(f16x2, w[i >> 1]);
     return i & 1 ? f16x2{t.y, t.y} : f16x2{t.x, t.x};
 }
-// one operation for (w & mask) | bits: of two constants one has to sit in a vector register, which the compiler does not choose by itself (it takes two operations)
-__device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t mask, uint32_t bits) {
-    uint32_t r;
-    asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(r) : "v"(w), "s"(mask), "v"(bits));
-    return r;
+// The four pairs of codes of a word, less 8: those at nibbles 0 and 2 over the bits of 1024, those at 1 and 3 are 1024 + 16 code. The masks are held in registers, one of them a vector
+// register: of two constants that it can see the compiler makes two operations instead of one v_and_or_b32.
+struct pm_masks { uint32_t even, odd, bits; };
+__device__ __forceinline__ pm_masks masks() {
+    pm_masks m{0x000f000fu, 0x00f000f0u, 0x64006400u};
+    asm("" : "+s"(m.even), "+s"(m.odd), "+v"(m.bits));
+    return m;
 }
-// the four pairs of codes of a word, less 8: those at nibbles 0 and 2 over the bits of 1024, those at 1 and 3 are 1024 + 16 code
-__device__ __forceinline__ void codes(uint32_t w, f16x2 * n) {
+__device__ __forceinline__ void codes(uint32_t w, const pm_masks & m, f16x2 * n) {
     const uint32_t u = w >> 8;
     const f16x2 zero = {(_Float16) -1032.0f, (_Float16) -1032.0f}, part = {(_Float16) 0.0625f, (_Float16) 0.0625f}, less = {(_Float16) -72.0f, (_Float16) -72.0f};
-    n[0] = __builtin_bit_cast(f16x2, and_or(w, 0x000f000fu, 0x64006400u)) + zero;
-    n[1] = __builtin_elementwise_fma(__builtin_bit_cast(f16x2, and_or(w, 0x00f000f0u, 0x64006400u)), part, less);
-    n[2] = __builtin_bit_cast(f16x2, and_or(u, 0x000f000fu, 0x64006400u)) + zero;
-    n[3] = __builtin_elementwise_fma(__builtin_bit_cast(f16x2, and_or(u, 0x00f000f0u, 0x64006400u)), part, less);
+    n[0] = __builtin_bit_cast(f16x2, (w & m.even) | m.bits) + zero;
+    n[1] = __builtin_elementwise_fma(__builtin_bit_cast(f16x2, (w & m.odd) | m.bits), part, less);
+    n[2] = __builtin_bit_cast(f16x2, (u & m.even) | m.bits) + zero;
+    n[3] = __builtin_elementwise_fma(__builtin_bit_cast(f16x2, (u & m.odd) | m.bits), part, less);
 }
 __device__ __forceinline__ f16x8 eight(f16x2 a, f16x2 b, f16x2 c, f16x2 d) { return f16x8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y}; }
 // scales beyond what the cache store makes (8188: its codes stay finite), NaN and infinities become 0; bits 0, 1: which
@@ -258,6 +259,7 @@ template <typename T, int NB, bool WIDE, int CT> __global__ __launch_bounds__(FW
             if (o < 64 * NB) { dma4(ks, o, to + Q::KS + j * 256); dma4(vs, (o >> 6) * (PM_PAGE * 2) + (o & 63), to + Q::VS + j * 256); }
         }
     };
+    const pm_masks mk = masks();
     int i = 2 * s * per + wave, page = page_of(i), next = page_of(i + FW), stage = 0;
     if (i < end) load(i, page, 0);
     if (i + FW < end) load(i + FW, next, 1);
@@ -314,7 +316,7 @@ template <typename T, int NB, bool WIDE, int CT> __global__ __launch_bounds__(FW
         for (int b = 0; b < NB; ++b) {
             const f16x2 sa = half_of(xs[0], b), sb = half_of(xs[1], b);
             f16x2 na[4], nb[4];
-            codes(xk[0][b], na); codes(xk[1][b], nb);
+            codes(xk[0][b], mk, na); codes(xk[1][b], mk, nb);
             const f16x8 ka = eight(na[0] * sa, na[1] * sa, na[2] * sa, na[3] * sa), kb = eight(nb[0] * sb, nb[1] * sb, nb[2] * sb, nb[3] * sb);
 #pragma unroll
             for (int u = 0; u < CT; ++u) {
@@ -372,7 +374,7 @@ template <typename T, int NB, bool WIDE, int CT> __global__ __launch_bounds__(FW
             f16x2 sc[4], na[4], nb[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) sc[j] = __builtin_bit_cast(f16x2, vs[w][j]);
-            codes(xv[0][w], na); codes(xv[1][w], nb);
+            codes(xv[0][w], mk, na); codes(xv[1][w], mk, nb);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const f16x8 v = eight(na[h] * sc[0], na[h + 2] * sc[1], nb[h] * sc[2], nb[h + 2] * sc[3]);
@@ -423,14 +425,15 @@ template <typename T, int NB, bool WIDE, int CT> __global__ __launch_bounds__(FW
 }
 
 // ---- prompts ----------------------------------------------------------------------------------------------------------------
+constexpr int AHEAD = 4;                                   // operands on their way from LDS
 constexpr int TC = 128;                                    // columns of a tile: 32 per wave
 
 template <typename T, int NB, bool WIDE> __global__ __launch_bounds__(256, NB <= 4 ? 2 : 1) void tiles_kernel(pm_kv4_cache c, pm_kv4_attn a, int splits) {
     constexpr int D = NB * 32, KS = D / 16, VT = D / 32, KL = D * 2 + 16, VL = PM_PAGE * 2 + 16;      // LDS rows are an odd number of 16-byte pieces: no bank is asked twice
     typedef pm_kv4_slab<NB> S;
-    extern __shared__ __attribute__((aligned(16))) char lds[];            // K [64][KL], V^T [D][VL]
-    char * k_l = lds, * v_l = lds + PM_PAGE * KL;
-    __shared__ uint8_t bad_l[16];
+    extern __shared__ __attribute__((aligned(16))) char lds[];            // two pages: K [64][KL], V^T [D][VL]
+    constexpr int STAGE = PM_PAGE * KL + D * VL;
+    __shared__ __attribute__((aligned(16))) uint8_t bad_l[2][16];
     const int G = c.G, R = a.H / G, g = blockIdx.x % G, s = blockIdx.y;
     const int at = a.n_tiles - 1 - (int) (blockIdx.x / G);                // (later tiles see more keys: they start first)
     const size_t slot = blockIdx.x;
@@ -451,17 +454,47 @@ template <typename T, int NB, bool WIDE> __global__ __launch_bounds__(256, NB <=
     auto page_of = [&](int i) __attribute__((always_inline)) { if (!known || i >= end) return -1; const int p = table[page_at(see, i)]; return (unsigned) p < (unsigned) c.n_pages ? p : -1; };
     // a page on its way: thread t has the codes of key row t / 4, dimensions 8 (t % 4) .. + 7 of each block, and of token quad t / 16, dimensions n and n + 16 of each block, n = t % 16
     const int kr = threadIdx.x >> 2, kg = threadIdx.x & 3, vq = threadIdx.x >> 4, vn = threadIdx.x & 15;
+    const pm_masks mk = masks();
     uint32_t xk[NB], xks[(NB + 1) / 2], xv[NB], xvs[NB][2];
-    auto load = [&](int page) __attribute__((always_inline)) {
-        if (page < 0) return;
-        const PM_G char * slab = (const PM_G char *) uniform_ptr((char *) head + (size_t) page * G * S::BYTES);
-        ld_words<NB>(slab + S::K + kr * 16 * NB + kg * 4 * NB, xk);
-        ld_halves<NB>(slab + S::KS + kr * 2 * NB, xks);
-        ld_words<NB>(slab + S::V + vq * 64 * NB + vn * 4 * NB, xv);
+    auto load = [&](int page) __attribute__((always_inline)) {             // (what is not there is read from page 0 and hidden)
+        const PM_G char * slab = (const PM_G char *) uniform_ptr((char *) head + (size_t) (page < 0 ? 0 : page) * G * S::BYTES);
+        ld_words<NB>(slab + S::K + (uint32_t) (kr * 16 * NB + kg * 4 * NB), xk);
+        ld_halves<NB>(slab + S::KS + (uint32_t) (kr * 2 * NB), xks);
+        ld_words<NB>(slab + S::V + (uint32_t) (vq * 64 * NB + vn * 4 * NB), xv);
 #pragma unroll
-        for (int w = 0; w < NB; ++w) ld_words<2>(slab + S::VS + (w * PM_PAGE + vq * 4) * 2, xvs[w]);
+        for (int w = 0; w < NB; ++w) ld_words<2>(slab + S::VS + w * PM_PAGE * 2 + (uint32_t) (vq * 8), xvs[w]);
     };
-    int page = page_of(begin);
+    // every column sees the page whole; else scales that are not finite are taken out of it
+    auto whole = [&](int i, int page) __attribute__((always_inline)) { const int key0 = page_at(see, i) * PM_PAGE; return page >= 0 && key0 + PM_PAGE - 1 <= see.lo && !(a.window > 0 && key0 <= see.hi - a.window); };
+    auto clean = [&](int stage) __attribute__((always_inline)) {
+        uint32_t bad = 0;
+#pragma unroll
+        for (int w = 0; w < NB; ++w) bad |= finite(xvs[w][0]) | finite(xvs[w][1]) << 2;
+        if (vn == 0) bad_l[stage][vq] = (uint8_t) bad;
+    };
+    // the page in registers as f16, in 4 NB pieces: key block b in pieces 2 b and 2 b + 1 (codes; scale and store), value block b in 2 NB + 2 b and the one behind it
+    f16x2 half_done[4];
+    auto expand = [&](int piece, int stage) __attribute__((always_inline)) {
+        const int b = piece / 2 % NB;
+        const bool val = piece >= 2 * NB;
+        if (piece % 2 == 0) { codes(val ? xv[b] : xk[b], mk, half_done); return; }
+        char * k_l = lds + stage * STAGE, * v_l = k_l + PM_PAGE * KL;
+        const f16x2 * n = half_done;
+        if (!val) {
+            const f16x2 sc = half_of(xks, b);
+            *(f16x8 *) (k_l + kr * KL + (b * 4 + kg) * 16) = eight(n[0] * sc, n[1] * sc, n[2] * sc, n[3] * sc);
+        } else {
+            const f16x2 s0 = __builtin_bit_cast(f16x2, xvs[b][0]), s1 = __builtin_bit_cast(f16x2, xvs[b][1]);
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                *(u32x2 *) (v_l + (b * 32 + h * 16 + vn) * VL + vq * 8) = u32x2{__builtin_bit_cast(uint32_t, n[h] * s0), __builtin_bit_cast(uint32_t, n[h + 2] * s1)};
+        }
+    };
+    auto expand_all = [&](int stage) __attribute__((always_inline)) {
+#pragma unroll
+        for (int q = 0; q < 4 * NB; ++q) expand(q, stage);
+    };
+    int page = page_of(begin), next = page_of(begin + 1);
     load(page);
 
     f16x8 qh[KS], ql[KS];
@@ -492,62 +525,60 @@ template <typename T, int NB, bool WIDE> __global__ __launch_bounds__(256, NB <=
         for (int e = 0; e < 16; ++e) acc[t][e] = 0.0f;
     float m = NONE, l = 0.0f;
     const int krow = (lr & 0x13) | (lr >> 3 & 1) << 2 | (lr >> 2 & 1) << 3;       // key of score row lr: bits 2 and 3 changed over
-    for (int i = begin; i < end; ++i) {
-        const int next = page_of(i + 1), key0 = page_at(see, i) * PM_PAGE;
-        const bool whole = key0 + PM_PAGE - 1 <= see.lo && !(a.window > 0 && key0 <= see.hi - a.window);      // every column sees the page whole
-        if (page >= 0) {
-            __syncthreads();                               // (the page before is read)
-            if (!whole) {
-                uint32_t bad = 0;
-#pragma unroll
-                for (int w = 0; w < NB; ++w) bad |= finite(xvs[w][0]) | finite(xvs[w][1]) << 2;
-                if (vn == 0) bad_l[vq] = (uint8_t) bad;
-            }
-#pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                const f16x2 sc = half_of(xks, b);
-                f16x2 n[4];
-                codes(xk[b], n);
-                *(f16x8 *) (k_l + kr * KL + (b * 4 + kg) * 16) = eight(n[0] * sc, n[1] * sc, n[2] * sc, n[3] * sc);
-                codes(xv[b], n);
-                const f16x2 s0 = __builtin_bit_cast(f16x2, xvs[b][0]), s1 = __builtin_bit_cast(f16x2, xvs[b][1]);
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-                    *(u32x2 *) (v_l + (b * 32 + h * 16 + vn) * VL + vq * 8) = u32x2{__builtin_bit_cast(uint32_t, n[h] * s0), __builtin_bit_cast(uint32_t, n[h + 2] * s1)};
-            }
-            __syncthreads();
-        }
+    if (begin < end) {
+        if (!whole(begin, page)) { asm volatile(""); clean(0); }
+        expand_all(0);
         load(next);
-        const bool go = page >= 0 && w_on && key0 <= w_hi;
-        page = next;
-        if (!go) continue;
+    }
+    // Two pages in LDS: while the scores of one are formed on the matrix cores, the vector pipe makes the next one f16; the products with the values run among the exponentials
+    for (int i = begin, stage = 0; i < end; ++i, stage ^= 1) {
+        const int after = page_of(i + 2), key0 = page_at(see, i) * PM_PAGE;
+        const bool all = whole(i, page), there = page >= 0;
+        if (i + 1 < end && !whole(i + 1, next)) { asm volatile(""); clean(stage ^ 1); }
+        page = next; next = after;
+        __syncthreads();                                   // (this page is there, the other stage is read)
+        const char * k_l = lds + stage * STAGE, * v_l = k_l + PM_PAGE * KL;
         f32x16 sc[2];
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
+        for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int e = 0; e < 16; ++e) sc[t][e] = 0.0f;
+        // a matrix instruction, its share of the vector work, and so on: in the order that stands here (the compiler would put the products together, which then wait for each other)
+        auto key = [&](int q) __attribute__((always_inline)) { return *(const f16x8 *) (k_l + (q / KS * 32 + krow) * KL + (q % KS * 2 + hf) * 16); };
+        f16x8 kf[AHEAD];
 #pragma unroll
-            for (int b = 0; b < KS; ++b) {
-                const f16x8 k = *(const f16x8 *) (k_l + (t * 32 + krow) * KL + (b * 2 + hf) * 16);
-                sc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qh[b], sc[t], 0, 0, 0);
-                if (WIDE) sc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, ql[b], sc[t], 0, 0, 0);
+        for (int q = 0; q < AHEAD; ++q) kf[q] = key(q);
+#pragma unroll
+        for (int q = 0; q < 2 * KS; ++q) {
+            const f16x8 k = kf[q % AHEAD];
+            if (q + AHEAD < 2 * KS) kf[q % AHEAD] = key(q + AHEAD);
+            sc[q / KS] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qh[q % KS], sc[q / KS], 0, 0, 0);
+            if (WIDE) sc[q / KS] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, ql[q % KS], sc[q / KS], 0, 0, 0);
+            expand(q, stage ^ 1);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        load(next);
+        if (!w_on || key0 > w_hi) continue;                // (a path of its own around the products too costs the registers of both)
+        if (!all) {
+            asm volatile("");
+            const int last = there ? pos : -1;
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const uint32_t bad = *(const uint16_t *) (bad_l[stage] + t * 4 + hf * 2);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int key = key0 + t * 16 + 8 * hf + e;
+                    const bool ok = key <= last && (key >= low || key < a.first);
+                    sc[t >> 1][(t & 1) * 8 + e] = ok ? (bad >> ((e >> 2) * 8 + (e & 3)) & 1 ? NAN : sc[t >> 1][(t & 1) * 8 + e]) : -INFINITY;
+                }
             }
         }
-        if (!whole)
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const int kk = t * 32 + 16 * (e >> 3) + 8 * hf + (e & 7), key = key0 + kk;
-                    const bool ok = key <= pos && (key >= low || key < a.first);
-                    sc[t][e] = ok ? (bad_l[kk >> 2] >> (kk & 3) & 1 ? NAN : sc[t][e]) : -INFINITY;
-                }
         float mx = sc[0][0];
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int e = 0; e < 16; ++e) mx = fmaxf(mx, sc[t][e]);
-        mx = fmaxf(fmaxf(mx, __shfl_xor(mx, 32)) * cf, NONE);
+        mx = fmaxf(fmaxf(mx, __builtin_bit_cast(float, other_half(__builtin_bit_cast(uint32_t, mx)))) * cf, NONE);
         if (__any(mx > m + SLACK)) {
             const float mn = fmaxf(m, mx), corr = __builtin_amdgcn_exp2f(m - mn);
             m = mn; l *= corr;
@@ -557,22 +588,36 @@ template <typename T, int NB, bool WIDE> __global__ __launch_bounds__(256, NB <=
                 for (int e = 0; e < 16; ++e) acc[t][e] *= corr;
         }
         const float mo = HELD - m;
+        f16x2 ph[2][4], pl[2][4];                          // probabilities of 16 keys, and of the next 16
+        auto weigh = [&](int j, int e) __attribute__((always_inline)) {
+            const float p = __builtin_amdgcn_exp2f(fmaf(sc[j >> 1][(j & 1) * 8 + 2 * e], cf, mo)), q = __builtin_amdgcn_exp2f(fmaf(sc[j >> 1][(j & 1) * 8 + 2 * e + 1], cf, mo));
+            l += p; l += q;
+            const f16x2 h = {(_Float16) p, (_Float16) q};
+            ph[j & 1][e] = h;
+            if (WIDE) pl[j & 1][e] = f16x2{(_Float16) (p - (float) h.x), (_Float16) (q - (float) h.y)};
+        };
+        auto value = [&](int q) __attribute__((always_inline)) { return *(const f16x8 *) (v_l + (q % VT * 32 + lr) * VL + (q / VT * 2 + hf) * 16); };
+        f16x8 vf[AHEAD];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            float p[8];
-            f16x8 ph, pl;
+        for (int q = 0; q < AHEAD; ++q) vf[q] = value(q);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) { p[e] = __builtin_amdgcn_exp2f(fmaf(sc[j >> 1][(j & 1) * 8 + e], cf, mo)); l += p[e]; }
-            split_f16(p, ph, pl);
+        for (int e = 0; e < 4; ++e) weigh(0, e);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int t = 0; t < VT; ++t) {
-                const f16x8 v = *(const f16x8 *) (v_l + (t * 32 + lr) * VL + (j * 2 + hf) * 16);
-                acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph, acc[t], 0, 0, 0);
-                if (WIDE) acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl, acc[t], 0, 0, 0);
-            }
+        for (int q = 0; q < 4 * VT; ++q) {
+            const int j = q / VT, t = q % VT;
+            const f16x2 * h = ph[j & 1], * w = pl[j & 1];
+            const f16x8 v = vf[q % AHEAD];
+            if (q + AHEAD < 4 * VT) vf[q % AHEAD] = value(q + AHEAD);
+            acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, eight(h[0], h[1], h[2], h[3]), acc[t], 0, 0, 0);
+            if (WIDE) acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, eight(w[0], w[1], w[2], w[3]), acc[t], 0, 0, 0);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) if (j < 3 && e * VT / 4 == t) weigh(j + 1, e);
+            __builtin_amdgcn_sched_barrier(0);
         }
     }
     l += __shfl_xor(l, 32);
+    __syncthreads();
     if (splits == 1) {
         if (!on) return;
         const float f = l == 0.0f ? 0.0f : 1.0f / l;
@@ -633,7 +678,7 @@ template <typename T, int NB> int launch(const pm_kv4_cache & c, pm_kv4_attn a, 
     }
     const int64_t slots = (int64_t) a.n_tiles * c.G;
     const int splits = splits_of(a, slots, slots, TILES_WANT, TILES_LEAST, TILES_MOST, TC * (D + 2));
-    const size_t stage = (size_t) PM_PAGE * (D * 2 + 16) + D * (PM_PAGE * 2 + 16), ml = splits > 1 ? (size_t) splits * TC * 8 + 4096 : 0, lds = stage > ml ? stage : ml;
+    const size_t stage = 2 * ((size_t) PM_PAGE * (D * 2 + 16) + D * (PM_PAGE * 2 + 16)), ml = splits > 1 ? (size_t) splits * TC * 8 + 4096 : 0, lds = stage > ml ? stage : ml;
     pm_allow_big_lds((const void *) tiles_kernel<T, NB, WIDE>, lds);
     hipLaunchKernelGGL((tiles_kernel<T, NB, WIDE>), dim3((unsigned) slots, splits), dim3(256), lds, st, c, a, splits);
     return 0;
