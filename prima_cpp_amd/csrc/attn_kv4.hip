@@ -10,6 +10,7 @@
 #include "pm355_kv4.h"
 #include "pm355_kernels.h"
 #include "../../include/prima_mi355.h"
+#include <type_traits>
 
 namespace {
 
@@ -22,7 +23,6 @@ typedef uint16_t u16x4 __attribute__((ext_vector_type(4)));
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float NONE = -1e30f;                             // running maximum before the first visible key
 constexpr float HELD = 8.0f, SLACK = 6.0f;                 // probabilities are held times 2^HELD; the running maximum may lag by SLACK (2^14 < 65504), sums are seldom rescaled
-constexpr int TICKETS = 65536;                             // words of the scratch in front of the partial sums
 
 // N words (N halves) that lie side by side, a multiple of 4 N (2 N) bytes into a slab
 template <int N> __device__ __forceinline__ void ld_words(const PM_G char * p, uint32_t * w) {
@@ -64,74 +64,6 @@ __device__ __forceinline__ uint32_t finite(uint32_t & s) {
     const uint32_t lo = (s & 0x7fffu) > 0x6fffu, hi = (s & 0x7fffffffu) > 0x6fffffffu;
     s &= (lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u);
     return lo | hi << 1;
-}
-// ---- partial sums of split keys: per slot [splits][COLS][D] and [splits][COLS][maximum, sum]; stores that every XCD sees once they are waited for
-__device__ __forceinline__ void put(float * p, float x, float y) {
-    __hip_atomic_store((PM_G uint64_t *) p, __builtin_bit_cast(uint64_t, f32x2{x, y}), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-__device__ __forceinline__ void put(float * p, f32x4 v) { put(p, v.x, v.y); put(p + 2, v.z, v.w); }
-// After put(): whether this workgroup is the last of its slot. Tickets count up to `splits` and go back to 0.
-__device__ __forceinline__ bool last_of(float * work, size_t slot, int splits) {
-    __shared__ int is_last;
-    pm_vm_drain();
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        unsigned * tk = (unsigned *) work + slot;
-        is_last = __hip_atomic_fetch_add(tk, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned) splits - 1;
-        if (is_last) __hip_atomic_store(tk, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
-    __syncthreads();
-    if (!is_last) return false;
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
-    return true;
-}
-// The last one joins the splits in their order (results do not depend on who that is): 4 dimensions of a column per thread, up to 16 splits on their way at once - a load that comes from
-// another XCD's store takes about a microsecond, and one at a time 128 splits took 40. lds: splits * COLS * 2 + 4 NT floats
-template <int D, int COLS, int NT, typename F> __device__ __forceinline__ void join(const float * part, int splits, int cols, float * lds, F && store) {
-    __shared__ float inv[COLS];
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const float * ml = part + (size_t) splits * COLS * D;
-    for (int o = threadIdx.x; o < splits * COLS; o += NT)
-        if (o % COLS < cols) { const f32x2 v = *(const PM_G f32x2 *) (ml + 2 * o); lds[2 * o] = v.x; lds[2 * o + 1] = v.y; }
-    __syncthreads();
-    for (int col = wave; col < cols; col += NT / 64) {           // maximum and sum of a column by a wave; the factors of its splits take the place of their maxima
-        float M = NONE, L = 0.0f;
-        for (int k = lane; k < splits; k += 64) M = fmaxf(M, lds[(k * COLS + col) * 2]);
-        M = all_max(M);
-        for (int k = lane; k < splits; k += 64) { const float f = __builtin_amdgcn_exp2f(lds[(k * COLS + col) * 2] - M); lds[(k * COLS + col) * 2] = f; L = fmaf(lds[(k * COLS + col) * 2 + 1], f, L); }
-        L = wave_sum(L);
-        if (lane == 0) inv[col] = L == 0.0f ? 0.0f : 1.0f / L;
-    }
-    __syncthreads();
-    const int items = cols * (D / 4), groups = items < NT ? NT / items : 1;
-    float * sums = lds + splits * COLS * 2;
-    for (int o = threadIdx.x; o < items * groups; o += NT) {
-        const int grp = o / items, it = o % items, col = it / (D / 4), d = it % (D / 4) * 4;
-        const float * p = part + (size_t) col * D + d;
-        f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int k0 = grp; k0 < splits; k0 += 16 * groups) {
-            f32x4 r[16];
-#pragma unroll
-            for (int k = 0; k < 16; ++k) { const int z = k0 + k * groups; r[k] = *(const PM_G f32x4 *) (p + (size_t) (z < splits ? z : splits - 1) * COLS * D); }
-#pragma unroll
-            for (int k = 0; k < 16; ++k) {
-                const int z = k0 + k * groups;
-                const float f = z < splits ? lds[(z * COLS + col) * 2] : 0.0f;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) if (z < splits) v[e] = fmaf(r[k][e], f, v[e]);
-            }
-        }
-        if (groups == 1) store(col, d, v * inv[col]);
-        else *(f32x4 *) (sums + o * 4) = v;
-    }
-    if (groups == 1) return;
-    __syncthreads();
-    for (int it = threadIdx.x; it < items; it += NT) {
-        f32x4 v = *(const f32x4 *) (sums + it * 4);
-        for (int k = 1; k < groups; ++k) v += *(const f32x4 *) (sums + (k * items + it) * 4);
-        const int col = it / (D / 4);
-        store(col, it % (D / 4) * 4, v * inv[col]);
-    }
 }
 template <typename T> __device__ __forceinline__ void st_out(T * p, f32x4 v) {
     if constexpr (sizeof(T) == 2) *(PM_G u16x4 *) p = u16x4{f2bf(v.x), f2bf(v.y), f2bf(v.z), f2bf(v.w)};
@@ -394,7 +326,7 @@ template <typename T, int NB, bool WIDE, int CT> __global__ __launch_bounds__(FW
         const int row = row0 + (col0 + col) / R;
         if ((unsigned) row < (unsigned) a.n_tokens) st_out((T *) a.out + (size_t) row * a.ldo + (g * R + (col0 + col) % R) * D + d, o);
     };
-    float * part = a.work + TICKETS + slot * splits * COLS * (D + 2);
+    float * part = a.work + slot * splits * COLS * (D + 2);
 #pragma unroll
     for (int u = 0; u < CT; ++u) {
         const int have = cols - u * 16 < 16 ? cols - u * 16 : 16;          // (may be none)
@@ -416,12 +348,11 @@ template <typename T, int NB, bool WIDE, int CT> __global__ __launch_bounds__(FW
             for (int w = 0; w < FW; ++w) { const float f = __builtin_amdgcn_exp2f(m_l[w][col] - M); v += *(const f32x4 *) (acc_l + (w * 16 + col) * LD + d) * f; sum += l_l[w][col] * f; }
             if (splits == 1) store(u * 16 + col, d, v * (sum == 0.0f ? 0.0f : 1.0f / sum));
             else {
-                put(part + (size_t) (s * COLS + u * 16 + col) * D + d, v);
-                if (d == 0) put(part + (size_t) splits * COLS * D + (s * COLS + u * 16 + col) * 2, M, sum);
+                *(PM_G f32x4 *) (part + (size_t) (s * COLS + u * 16 + col) * D + d) = v;
+                if (d == 0) *(PM_G f32x2 *) (part + (size_t) splits * COLS * D + (s * COLS + u * 16 + col) * 2) = f32x2{M, sum};
             }
         }
     }
-    if (splits > 1 && last_of(a.work, slot, splits)) join<D, COLS, FW * 64>(part, splits, cols, acc_l, store);
 }
 
 // ---- prompts ----------------------------------------------------------------------------------------------------------------
@@ -436,7 +367,7 @@ template <typename T, int NB, bool WIDE> __global__ __launch_bounds__(256, NB <=
     __shared__ __attribute__((aligned(16))) uint8_t bad_l[2][16];
     const int G = c.G, R = a.H / G, g = blockIdx.x % G, s = blockIdx.y;
     const int at = a.n_tiles - 1 - (int) (blockIdx.x / G);                // (later tiles see more keys: they start first)
-    const size_t slot = blockIdx.x;
+    const size_t slot = (size_t) at * G + g;
     const int32_t * tile = uniform_const_ptr(a.tiles) + (size_t) at * 4;
     const int row0 = tile[0], seq = tile[3], pos0 = tile[2] < 0x7fffff00 ? tile[2] : 0x7fffff00, n = tile[1] < a.tile_tokens ? tile[1] : a.tile_tokens;
     if (n < 1) return;
@@ -628,33 +559,105 @@ template <typename T, int NB, bool WIDE> __global__ __launch_bounds__(256, NB <=
             for (int e = 0; e < 16; e += 4) st_out(o + t * 32 + 2 * e + 4 * hf, f32x4{acc[t][e], acc[t][e + 1], acc[t][e + 2], acc[t][e + 3]} * f);
         return;
     }
-    float * part = a.work + TICKETS + slot * splits * TC * (D + 2);
-    if (col < cols) {
-        float * r = part + ((size_t) s * TC + col) * D;
+    float * part = a.work + slot * splits * TC * (D + 2);
+    // (through LDS: a lane holds pieces of one column, memory wants whole lines)
+    constexpr int LD = D + 4;
+    float * sums = (float *) lds + wave * 32 * LD;
 #pragma unroll
-        for (int t = 0; t < VT; ++t)
+    for (int t = 0; t < VT; ++t)
 #pragma unroll
-            for (int e = 0; e < 16; e += 4) put(r + t * 32 + 2 * e + 4 * hf, f32x4{acc[t][e], acc[t][e + 1], acc[t][e + 2], acc[t][e + 3]});
-        if (hf == 0) put(part + (size_t) splits * TC * D + (s * TC + col) * 2, m, l);
+        for (int e = 0; e < 16; e += 4) *(f32x4 *) (sums + lr * LD + t * 32 + 2 * e + 4 * hf) = f32x4{acc[t][e], acc[t][e + 1], acc[t][e + 2], acc[t][e + 3]};
+    if (hf == 0 && col < cols) *(PM_G f32x2 *) (part + (size_t) splits * TC * D + (s * TC + col) * 2) = f32x2{m, l};
+    __syncthreads();
+    for (int o = threadIdx.x; o < cols * (D / 4); o += 256)
+        *(PM_G f32x4 *) (part + (size_t) s * TC * D + o * 4) = *(const f32x4 *) ((const float *) lds + o / (D / 4) * LD + o % (D / 4) * 4);
+}
+
+// ---- joining split keys: partial sums per slot [splits][COLS][D], then [splits][COLS][maximum, sum]. A launch of its own: the workgroup of a slot that ends last could do it too, but it
+// reads 2 MB (128 columns, 32 splits) alone, and waits for three trips to memory that other XCDs have written to; 64 tokens behind 30000 took 118 us that way ------------------------------
+template <typename T, int D, int COLS> __global__ __launch_bounds__(256) void join_kernel(pm_kv4_cache c, pm_kv4_attn a, int passes, int splits, int each) {
+    extern __shared__ __attribute__((aligned(16))) char lds_j[];          // [splits][each][factor, sum], then the sums of groups of splits
+    __shared__ float inv[COLS];
+    float * ml = (float *) lds_j, * sums = ml + splits * each * 2;
+    const int blocks = (COLS + each - 1) / each, first = blockIdx.x % blocks * each, G = c.G, R = a.H / G;
+    const size_t slot = blockIdx.x / blocks;
+    const int g = slot % G, pass = slot / G % passes;
+    const int32_t * tile = uniform_const_ptr(a.tiles) + slot / G / passes * 4;
+    const int row0 = tile[0], n = tile[1] < a.tile_tokens ? tile[1] : a.tile_tokens, room = COLS - first < each ? COLS - first : each, left = n * R - pass * COLS - first, cols = left < room ? left : room;
+    if (cols < 1) return;
+    const float * part = a.work + slot * splits * COLS * (D + 2) + first * D, * part_ml = a.work + slot * splits * COLS * (D + 2) + (size_t) splits * COLS * D + first * 2;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, items = cols * (D / 4), groups = items < 256 ? 256 / items : 1;
+    // the first splits of this thread's column are on their way while the factors are formed
+    constexpr int KB = 16;
+    const int it0 = threadIdx.x % items, grp = groups > 1 ? threadIdx.x / items : 0;
+    f32x4 r[KB];
+    auto fetch = [&](int it, int k0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int k = 0; k < KB; ++k) {
+            const int z = k0 + k * groups < splits ? k0 + k * groups : splits - 1;
+            r[k] = *(const PM_G f32x4 *) (part + ((size_t) z * COLS + it / (D / 4)) * D + it % (D / 4) * 4);
+        }
+    };
+    fetch(it0, grp);
+    for (int o = threadIdx.x; o < splits * cols; o += 256) {
+        const f32x2 v = *(const PM_G f32x2 *) (part_ml + (o / cols * COLS + o % cols) * 2);
+        ml[(o / cols * each + o % cols) * 2] = v.x; ml[(o / cols * each + o % cols) * 2 + 1] = v.y;
     }
-    if (last_of(a.work, slot, splits))
-        join<D, TC, 256>(part, splits, cols, (float *) lds, [&](int k, int d, f32x4 o) {
-            const int to = row0 + k / R;
-            if ((unsigned) to < (unsigned) a.n_tokens) st_out((T *) a.out + (size_t) to * a.ldo + (g * R + k % R) * D + d, o);
-        });
+    __syncthreads();
+    for (int col = wave; col < cols; col += 4) {           // maximum and sum of a column by a wave; the factors of its splits take the place of their maxima
+        float M = NONE, L = 0.0f;
+        for (int k = lane; k < splits; k += 64) M = fmaxf(M, ml[(k * each + col) * 2]);
+        M = all_max(M);
+        for (int k = lane; k < splits; k += 64) { const float f = __builtin_amdgcn_exp2f(ml[(k * each + col) * 2] - M); ml[(k * each + col) * 2] = f; L = fmaf(ml[(k * each + col) * 2 + 1], f, L); }
+        L = wave_sum(L);
+        if (lane == 0) inv[col] = L == 0.0f ? 0.0f : 1.0f / L;
+    }
+    __syncthreads();
+    auto store = [&](int it, f32x4 v) __attribute__((always_inline)) {
+        const int k = pass * COLS + first + it / (D / 4), row = row0 + k / R;
+        if ((unsigned) row < (unsigned) a.n_tokens) st_out((T *) a.out + (size_t) row * a.ldo + (g * R + k % R) * D + it % (D / 4) * 4, v * inv[it / (D / 4)]);
+    };
+    for (int o = threadIdx.x; o < items * groups; o += 256) {
+        const int it = o % items;
+        f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int k0 = grp; k0 < splits; k0 += KB * groups) {
+            if (o != (int) threadIdx.x || k0 != grp) fetch(it, k0);
+#pragma unroll
+            for (int k = 0; k < KB; ++k)
+                if (k0 + k * groups < splits) {
+                    const float f = ml[((k0 + k * groups) * each + it / (D / 4)) * 2];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] = fmaf(r[k][e], f, v[e]);
+                }
+        }
+        if (groups == 1) store(it, v);
+        else *(f32x4 *) (sums + o * 4) = v;
+    }
+    if (groups == 1) return;
+    __syncthreads();
+    for (int it = threadIdx.x; it < items; it += 256) {
+        f32x4 v = *(const f32x4 *) (sums + it * 4);
+        for (int k = 1; k < groups; ++k) v += *(const f32x4 *) (sums + (k * items + it) * 4);
+        store(it, v);
+    }
 }
 
 constexpr int FEW_WANT = 256, FEW_LEAST = 4, FEW_MOST = 128, FEW_COLS = 48, TILES_WANT = 512, TILES_LEAST = 8, TILES_MOST = 32;
 // workgroups over which the keys of a slot are split: as many as fill the chip, none with less than `least` pages, and what the scratch holds
 int splits_of(const pm_kv4_attn & a, int64_t slots, int64_t busy, int want, int least, int most, int64_t floats) {
-    const int64_t pages = ((int64_t) a.max_keys + PM_PAGE - 1) / PM_PAGE, room = a.work && a.work_floats > TICKETS ? (int64_t) (a.work_floats - TICKETS) / (slots * floats) : 1;
+    const int64_t pages = ((int64_t) a.max_keys + PM_PAGE - 1) / PM_PAGE, room = a.work ? (int64_t) a.work_floats / (slots * floats) : 1;
     int64_t n = (want + busy - 1) / busy;
     n = n < pages / least ? n : pages / least;
     n = n < room ? n : room;
     n = n < most ? n : most;
-    return slots > TICKETS || n < 1 ? 1 : (int) n;
+    return n < 1 ? 1 : (int) n;
 }
 
+// columns per workgroup: the joined values of a thread come from about 16 splits
+template <typename T, int D, int COLS> void join(const pm_kv4_cache & c, const pm_kv4_attn & a, int64_t slots, int passes, int splits, hipStream_t st) {
+    const int most = 1024 / D, want = 16384 / (D * splits), each = want < 1 ? 1 : want < most ? want : most;
+    hipLaunchKernelGGL((join_kernel<T, D, COLS>), dim3((unsigned) (slots * ((COLS + each - 1) / each))), dim3(256), (size_t) splits * each * 8 + 4096, st, c, a, passes, splits, each);
+}
 template <typename T, int NB> int launch(const pm_kv4_cache & c, pm_kv4_attn a, hipStream_t st) {
     constexpr int D = NB * 32;
     constexpr bool WIDE = sizeof(T) == 4;
@@ -662,32 +665,35 @@ template <typename T, int NB> int launch(const pm_kv4_cache & c, pm_kv4_attn a, 
     if (a.window > 0) { const int64_t most = (int64_t) a.window + a.tile_tokens + 128 + a.first; if (most < a.max_keys) a.max_keys = (int) most; }
     // columns of a tile on the average: tile_tokens only bounds them
     const int64_t cols = (int64_t) R * (a.n_tokens / a.n_tiles < a.tile_tokens ? (a.n_tokens + a.n_tiles - 1) / a.n_tiles : a.tile_tokens);
-    auto few = [&](auto kern, int ct) {
+    auto few = [&](auto kern, auto ctc) {
+        constexpr int ct = decltype(ctc)::value;
         const int passes = (R * a.tile_tokens + 16 * ct - 1) / (16 * ct);
         const int64_t slots = (int64_t) a.n_tiles * c.G * passes, busy = (int64_t) a.n_tiles * c.G * ((cols + 16 * ct - 1) / (16 * ct));
         const int splits = splits_of(a, slots, busy, FEW_WANT, FEW_LEAST, FEW_MOST, 16 * ct * (D + 2));
-        const size_t ring = (size_t) FW * STAGES * pm_step<NB>::BYTES, acc = (size_t) FW * 16 * (D + 4) * 4, ml = splits > 1 ? (size_t) splits * 16 * ct * 8 + FW * 64 * 16 : 0;
-        const size_t lds = ring > acc ? (ring > ml ? ring : ml) : acc > ml ? acc : ml;
+        const size_t ring = (size_t) FW * STAGES * pm_step<NB>::BYTES, acc = (size_t) FW * 16 * (D + 4) * 4, lds = ring > acc ? ring : acc;
         pm_allow_big_lds((const void *) kern, lds);
         hipLaunchKernelGGL(kern, dim3((unsigned) (slots * splits)), dim3(FW * 64), lds, st, c, a, passes, splits);
+        if (splits > 1) join<T, D, 16 * ct>(c, a, slots, passes, splits, st);
         return 0;
     };
     if (a.tile_tokens == 1 || cols <= FEW_COLS) {
-        if constexpr (NB <= (WIDE ? 3 : 4)) if (cols > 16) return few(few_kernel<T, NB, WIDE, 2>, 2);
-        return few(few_kernel<T, NB, WIDE, 1>, 1);
+        if constexpr (NB <= (WIDE ? 3 : 4)) if (cols > 16) return few(few_kernel<T, NB, WIDE, 2>, std::integral_constant<int, 2>());
+        return few(few_kernel<T, NB, WIDE, 1>, std::integral_constant<int, 1>());
     }
     const int64_t slots = (int64_t) a.n_tiles * c.G;
     const int splits = splits_of(a, slots, slots, TILES_WANT, TILES_LEAST, TILES_MOST, TC * (D + 2));
-    const size_t stage = 2 * ((size_t) PM_PAGE * (D * 2 + 16) + D * (PM_PAGE * 2 + 16)), ml = splits > 1 ? (size_t) splits * TC * 8 + 4096 : 0, lds = stage > ml ? stage : ml;
+    const size_t lds = 2 * ((size_t) PM_PAGE * (D * 2 + 16) + D * (PM_PAGE * 2 + 16));
+    static_assert(2 * (PM_PAGE * (D * 2 + 16) + D * (PM_PAGE * 2 + 16)) >= TC * (D + 4) * 4, "the partial sums go through the pages' LDS");
     pm_allow_big_lds((const void *) tiles_kernel<T, NB, WIDE>, lds);
     hipLaunchKernelGGL((tiles_kernel<T, NB, WIDE>), dim3((unsigned) slots, splits), dim3(256), lds, st, c, a, splits);
+    if (splits > 1) join<T, D, TC>(c, a, slots, 1, splits, st);
     return 0;
 }
 
 } // namespace
 
 // (slots * splits < want + slots, and slots < want where there are splits)
-size_t pm_kv4_work_floats(int H, int G, int d) { return TICKETS + (size_t) 2 * TILES_WANT * TC * (d + 2); }
+size_t pm_kv4_work_floats(int H, int G, int d) { return (size_t) 2 * TILES_WANT * TC * (d + 2); }
 int pm_launch_attn_kv4(const pm_kv4_cache & c, const pm_kv4_attn & a, hipStream_t st) {
 #define PM_CALL(NB) return a.type == PM_BF16 ? launch<uint16_t, NB>(c, a, st) : launch<float, NB>(c, a, st)
     switch (c.d) { case 64: PM_CALL(2); case 96: PM_CALL(3); case 128: PM_CALL(4); case 192: PM_CALL(6); case 256: PM_CALL(8); }
