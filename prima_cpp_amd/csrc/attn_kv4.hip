@@ -146,8 +146,8 @@ __device__ __forceinline__ uint32_t swizzled() {
     const uint32_t n = gridDim.x, x = blockIdx.x & 7, q = n >> 3, r = n & 7;
     return x * q + (x < r ? x : r) + (blockIdx.x >> 3);
 }
-// CT column tiles of 16 per workgroup share the keys' way from codes to f16; `passes` workgroups take the columns of a tile
-template <typename T, int NB, bool WIDE, int CT> __global__ __launch_bounds__(FW * 64, NB * CT <= 4 && !WIDE ? 4 : 2) void few_kernel(pm_kv4_cache c, pm_kv4_attn a, int passes, int splits) {
+// CT column tiles of 16 per workgroup share the keys' way from codes to f16; `launched` workgroups take the columns of a tile
+template <typename T, int NB, bool WIDE, int CT> __global__ __launch_bounds__(FW * 64, NB <= 4 && CT == 1 && !WIDE ? 4 : 2) void few_kernel(pm_kv4_cache c, pm_kv4_attn a, int launched, int passes, int splits) {
     constexpr int D = NB * 32, VT = D / 16, LD = D + 4, COLS = 16 * CT;
     typedef pm_kv4_slab<NB> S;
     typedef pm_step<NB> Q;
@@ -155,13 +155,17 @@ template <typename T, int NB, bool WIDE, int CT> __global__ __launch_bounds__(FW
     float * acc_l = (float *) lds;
     __shared__ float m_l[FW][16], l_l[FW][16];
     const uint32_t id = swizzled();
-    const int G = c.G, R = a.H / G, g = id % G, pass = id / G % passes, s = id / G / passes % splits, at = id / G / passes / splits;
-    const size_t slot = ((size_t) at * passes + pass) * G + g;
+    const int G = c.G, R = a.H / G, g = id % G, s = id / G / launched % splits, at = id / G / launched / splits;
     const int32_t * tile = uniform_const_ptr(a.tiles) + (size_t) at * 4;
     const int row0 = tile[0], seq = tile[3], pos0 = tile[2] < 0x7fffff00 ? tile[2] : 0x7fffff00, n = tile[1] < a.tile_tokens ? tile[1] : a.tile_tokens;
-    const int col0 = pass * COLS, left = n * R - col0, cols = left < COLS ? left : COLS;
-    if (n < 1 || cols < 1) return;
     const int wave = __builtin_amdgcn_readfirstlane((int) threadIdx.x >> 6), lane = threadIdx.x & 63, lr = lane & 15, lg = lane >> 4;
+    // (tiles may have more columns than they have on the average, for which the launch is made: with CT > 1 a workgroup takes the further ones too. Workgroups without work are no way
+    // out: each waits for its LDS behind those that work)
+    int pass = id / G % launched;
+    if (pass * COLS >= n * R) return;
+    do {
+    const size_t slot = ((size_t) at * passes + pass) * G + g;
+    const int col0 = pass * COLS, left = n * R - col0, cols = left < COLS ? left : COLS;
     const int t0 = col0 / R, tn = (col0 + cols - 1) / R - t0 + 1;          // tokens of the columns
     const pm_seen see = seen_by(c, a, pos0 < 0 ? -1 : pos0 + t0, tn);
     const int per = (see.count + splits - 1) / splits, end = 2 * ((s + 1) * per < see.count ? (s + 1) * per : see.count);
@@ -353,6 +357,9 @@ template <typename T, int NB, bool WIDE, int CT> __global__ __launch_bounds__(FW
             }
         }
     }
+    __syncthreads();
+    pass += launched;
+    } while (CT > 1 && pass * COLS < n * R);
 }
 
 // ---- prompts ----------------------------------------------------------------------------------------------------------------
@@ -642,7 +649,7 @@ template <typename T, int D, int COLS> __global__ __launch_bounds__(256) void jo
     }
 }
 
-constexpr int FEW_WANT = 256, FEW_LEAST = 4, FEW_MOST = 128, FEW_COLS = 48, TILES_WANT = 512, TILES_LEAST = 8, TILES_MOST = 32;
+constexpr int FEW_WANT = 256, FEW_LEAST = 4, FEW_MOST = 128, FEW_COLS = 64, TILES_WANT = 512, TILES_LEAST = 8, TILES_MOST = 32;
 // workgroups over which the keys of a slot are split: as many as fill the chip, none with less than `least` pages, and what the scratch holds
 int splits_of(const pm_kv4_attn & a, int64_t slots, int64_t busy, int want, int least, int most, int64_t floats) {
     const int64_t pages = ((int64_t) a.max_keys + PM_PAGE - 1) / PM_PAGE, room = a.work ? (int64_t) a.work_floats / (slots * floats) : 1;
@@ -667,12 +674,12 @@ template <typename T, int NB> int launch(const pm_kv4_cache & c, pm_kv4_attn a, 
     const int64_t cols = (int64_t) R * (a.n_tokens / a.n_tiles < a.tile_tokens ? (a.n_tokens + a.n_tiles - 1) / a.n_tiles : a.tile_tokens);
     auto few = [&](auto kern, auto ctc) {
         constexpr int ct = decltype(ctc)::value;
-        const int passes = (R * a.tile_tokens + 16 * ct - 1) / (16 * ct);
-        const int64_t slots = (int64_t) a.n_tiles * c.G * passes, busy = (int64_t) a.n_tiles * c.G * ((cols + 16 * ct - 1) / (16 * ct));
+        const int passes = (R * a.tile_tokens + 16 * ct - 1) / (16 * ct), launched = ct > 1 ? (int) ((cols + 16 * ct - 1) / (16 * ct)) : passes;
+        const int64_t slots = (int64_t) a.n_tiles * c.G * passes, busy = (int64_t) a.n_tiles * c.G * launched;
         const int splits = splits_of(a, slots, busy, FEW_WANT, FEW_LEAST, FEW_MOST, 16 * ct * (D + 2));
         const size_t ring = (size_t) FW * STAGES * pm_step<NB>::BYTES, acc = (size_t) FW * 16 * (D + 4) * 4, lds = ring > acc ? ring : acc;
         pm_allow_big_lds((const void *) kern, lds);
-        hipLaunchKernelGGL(kern, dim3((unsigned) (slots * splits)), dim3(FW * 64), lds, st, c, a, passes, splits);
+        hipLaunchKernelGGL(kern, dim3((unsigned) (busy * splits)), dim3(FW * 64), lds, st, c, a, launched, passes, splits);
         if (splits > 1) join<T, D, 16 * ct>(c, a, slots, passes, splits, st);
         return 0;
     };
