@@ -629,7 +629,6 @@ class AttnKV4Args(L.C.Structure):
 
 # the three structures in one call each (a decoded token's launch is a few microseconds: building ctypes structures field by field would take as long)
 _KV4_CACHE, _KV4_APPEND, _ATTN_KV4 = struct.Struct("@iiiPPii"), struct.Struct("@iiiPqPqiPPfPiifPP"), struct.Struct("@iiPqPqfiiPiiiiPN")
-_ACT = (torch.float32, torch.bfloat16)
 _ACT_TYPE = {torch.float32: F32, torch.bfloat16: L.BF16}
 _KV4_DIMS = (64, 96, 128, 192, 256)
 _kv4_calls = {}
@@ -653,11 +652,6 @@ def _same_device(*tensors):
     return device
 
 
-def _want(ok, what):
-    if not ok:
-        raise L.PM355Error(what)
-
-
 def kv4_page_bytes(n_head_kv, head_dim):
     """bytes of a 64-token page of one layer: 4.5 bits per value"""
     n = L.declare("pm355_kv4_page_bytes", _sz, [_i32, _i32])(n_head_kv, head_dim)
@@ -669,22 +663,33 @@ def kv4_page_bytes(n_head_kv, head_dim):
 def _kv4_cache(pages, table, n_head_kv, head_dim):
     if head_dim not in _KV4_DIMS or n_head_kv < 1:
         kv4_page_bytes(n_head_kv, head_dim)
-    size, (rows, cols) = n_head_kv * head_dim * 72, table.shape if table.dim() == 2 else (0, 0)
-    _want(pages.dtype is torch.uint8 and pages.dim() == 2 and pages.shape[1] == size and pages.is_contiguous(), "pages: contiguous uint8 [pages, %d] is wanted" % size)
-    _want(table.dtype is torch.int32 and rows and cols and table.is_contiguous(), "table: contiguous int32 rows of page numbers, one per sequence, are wanted")
-    return _KV4_CACHE.pack(n_head_kv, head_dim, pages.shape[0], pages.data_ptr(), table.data_ptr(), cols, rows)
+    size, shape, of = n_head_kv * head_dim * 72, pages.shape, table.shape
+    if not (pages.dtype is torch.uint8 and len(shape) == 2 and shape[1] == size and pages.is_contiguous()):
+        raise L.PM355Error("pages: contiguous uint8 [pages, %d] is wanted" % size)
+    if not (table.dtype is torch.int32 and len(of) == 2 and of[0] and of[1] and table.is_contiguous()):
+        raise L.PM355Error("table: contiguous int32 rows of page numbers, one per sequence, are wanted")
+    return _KV4_CACHE.pack(n_head_kv, head_dim, shape[0], pages.data_ptr(), table.data_ptr(), of[1], of[0])
 
 
 def _per_token(name, t, n):
-    _want(t.dtype is torch.int32 and t.dim() == 1 and t.shape[0] == n and (n < 2 or t.stride(0) == 1), "%s: %d contiguous int32 are wanted" % (name, n))
+    if not (t.dtype is torch.int32 and t.shape == (n,) and t.is_contiguous()):
+        raise L.PM355Error("%s: %d contiguous int32 are wanted" % (name, n))
     return t.data_ptr()
 
 
-def _rows(name, t, n, width, dtypes, unit):
+def _rows(name, t, n, width, unit):
     """(pointer, values between rows) of [n, >= width] whose rows start at multiples of `unit` values"""
-    shape, (ld, one) = t.shape, t.stride() if t.dim() == 2 else (0, 0)
-    _want(len(shape) == 2 and shape[0] == n and shape[1] >= width and t.dtype in dtypes and one == 1, "%s: %d rows of %d contiguous values in %s are wanted" % (name, n, width, " or ".join(str(d) for d in dtypes)))
-    return t.data_ptr(), ld if n > 1 else width + -width % unit
+    shape = t.shape
+    if not (len(shape) == 2 and shape[0] == n and shape[1] >= width and t.stride(1) == 1):
+        raise L.PM355Error("%s: %d rows of %d contiguous values are wanted" % (name, n, width))
+    return t.data_ptr(), t.stride(0) if n > 1 else width + -width % unit
+
+
+def _act(name, t):
+    ty = _ACT_TYPE.get(t.dtype)
+    if ty is None:
+        raise L.PM355Error("%s: float32 or bfloat16 is wanted" % name)
+    return ty
 
 
 def rope_turns(n_dims, n_ctx_orig=8192, freq_base=10000.0, freq_scale=1.0, ext_factor=0.0, attn_factor=1.0, beta_fast=32.0, beta_slow=1.0, freq_factors=None):
@@ -703,19 +708,28 @@ def kv4_append(proj, pages, table, pos, seq, n_head, n_head_kv, head_dim, q=None
     """Queries normed and rotated (returned, [T, n_head * head_dim] in the type of proj), keys likewise and values into 4-bit pages. proj [T, >= (n_head + 2 n_head_kv) * head_dim] rows
     q | k | v, f32 or bf16; pages uint8 [n, kv4_page_bytes()], table int32 [sequences, pages of a sequence], pos, seq int32 [T]; turns (rope_turns): None rotates nothing."""
     device = _same_device(proj, pages, table, pos, seq, q, norm_q, norm_k, turns)
-    c = _kv4_cache(pages, table, n_head_kv, head_dim)
-    T, dtype = proj.shape[0], proj.dtype
-    at, ld = _rows("proj", proj, T, (n_head + 2 * n_head_kv) * head_dim, _ACT, 4)
+    c, ty, T, dtype, width = _kv4_cache(pages, table, n_head_kv, head_dim), _act("proj", proj), proj.shape[0], proj.dtype, n_head * head_dim
+    at, ld = _rows("proj", proj, T, width + 2 * n_head_kv * head_dim, 4)
     if q is None:
-        q = torch.empty(T, n_head * head_dim, dtype=dtype, device=proj.device)
-    q_at, ldq = _rows("q", q, T, n_head * head_dim, (dtype,), 4)
-    for w in (norm_q, norm_k):
-        _want(w is None or (norm and w.dtype is torch.float32 and w.dim() == 1 and w.shape[0] == head_dim and w.stride(0) == 1), "norm weights: norm=True and %d contiguous float32 are wanted" % head_dim)
-    _want(turns is None or (turns.dtype is torch.float64 and turns.dim() == 1 and turns.is_contiguous()), "turns: contiguous float64 (rope_turns) is wanted")
+        q = torch.empty(T, width, dtype=dtype, device=proj.device)
+        q_at, ldq = q.data_ptr(), width
+    elif q.dtype is not dtype:
+        raise L.PM355Error("q: the type of proj is wanted")
+    else:
+        q_at, ldq = _rows("q", q, T, width, 4)
+    w_q = w_k = n_rot = t_at = 0
+    if norm_q is not None or norm_k is not None:
+        for w in (norm_q, norm_k):
+            if w is not None and not (norm and w.dtype is torch.float32 and w.shape == (head_dim,) and w.stride(0) == 1):
+                raise L.PM355Error("norm weights: norm=True and %d contiguous float32 are wanted" % head_dim)
+        w_q, w_k = ptr(norm_q) or 0, ptr(norm_k) or 0
+    if turns is not None:
+        if not (turns.dtype is torch.float64 and turns.dim() == 1 and turns.is_contiguous()):
+            raise L.PM355Error("turns: contiguous float64 (rope_turns) is wanted")
+        t_at, n_rot = turns.data_ptr(), 2 * turns.shape[0]
     pos, seq = _per_token("pos", pos, T), _per_token("seq", seq, T)
     if T:
-        _kv4_call("pm355_kv4_append", c, _KV4_APPEND.pack(_ACT_TYPE[dtype], n_head, T, at, ld, q_at, ldq, norm, ptr(norm_q) or 0, ptr(norm_k) or 0, eps, ptr(turns) or 0,
-                                                          0 if turns is None else 2 * turns.shape[0], neox, mscale, pos, seq), torch._C._cuda_getCurrentRawStream(device))
+        _kv4_call("pm355_kv4_append", c, _KV4_APPEND.pack(ty, n_head, T, at, ld, q_at, ldq, norm, w_q, w_k, eps, t_at, n_rot, neox, mscale, pos, seq), torch._C._cuda_getCurrentRawStream(device))
     return q
 
 
@@ -752,17 +766,25 @@ def attn_kv4(q, pages, table, tiles, tile_tokens, max_keys, n_head, n_head_kv, h
     """Attention of q [T, n_head * head_dim] (f32 or bf16) over 4-bit pages: causal, with window > 0 only the last `window` keys and the first n_first. tiles int32 [n, 4] {row, tokens,
     position, sequence} (kv4_tiles). Returns out, of which the rows that tiles name are written. work: kv4_work(), for one call at a time."""
     device = _same_device(q, pages, table, tiles, out, work)
-    c = _kv4_cache(pages, table, n_head_kv, head_dim)
-    T, n = q.shape[0], tiles.shape[0]
-    q_at, ldq = _rows("q", q, T, n_head * head_dim, _ACT, 8)
-    _want(tiles.dtype is torch.int32 and tiles.dim() == 2 and tiles.shape[1] == 4 and tiles.is_contiguous(), "tiles: contiguous int32 rows of 4 are wanted")
-    _want(work is None or (work.dtype is torch.float32 and work.is_contiguous()), "work: contiguous float32 is wanted")
+    c, ty, dtype, T, of, width = _kv4_cache(pages, table, n_head_kv, head_dim), _act("q", q), q.dtype, q.shape[0], tiles.shape, n_head * head_dim
+    q_at, ldq = _rows("q", q, T, width, 8)
+    if not (tiles.dtype is torch.int32 and len(of) == 2 and of[1] == 4 and tiles.is_contiguous()):
+        raise L.PM355Error("tiles: contiguous int32 rows of 4 are wanted")
+    w_at = w_n = 0
+    if work is not None:
+        if work.dtype is not torch.float32 or not work.is_contiguous():
+            raise L.PM355Error("work: contiguous float32 is wanted")
+        w_at, w_n = work.data_ptr(), work.numel()
     if out is None:
-        out = torch.empty(T, n_head * head_dim, dtype=q.dtype, device=q.device)
-    out_at, ldo = _rows("out", out, T, n_head * head_dim, (q.dtype,), 8)
-    if T and n:
-        _kv4_call("pm355_attn_kv4", c, _ATTN_KV4.pack(_ACT_TYPE[q.dtype], n_head, q_at, ldq, out_at, ldo, scale, window, n_first, tiles.data_ptr(), n, tile_tokens, max_keys, T,
-                                                      0 if work is None else work.data_ptr(), 0 if work is None else work.numel()), torch._C._cuda_getCurrentRawStream(device))
+        out = torch.empty(T, width, dtype=dtype, device=q.device)
+        out_at, ldo = out.data_ptr(), width
+    elif out.dtype is not dtype:
+        raise L.PM355Error("out: the type of q is wanted")
+    else:
+        out_at, ldo = _rows("out", out, T, width, 8)
+    if T and of[0]:
+        _kv4_call("pm355_attn_kv4", c, _ATTN_KV4.pack(ty, n_head, q_at, ldq, out_at, ldo, scale, window, n_first, tiles.data_ptr(), of[0], tile_tokens, max_keys, T, w_at, w_n),
+                  torch._C._cuda_getCurrentRawStream(device))
     return out
 
 
@@ -773,8 +795,10 @@ def pages_copy(pages, pairs):
     shape, stride = pages.shape, pages.stride()
     if len(shape) == 2:
         shape, stride = (1, *shape), (0, *stride)
-    _want(len(shape) == 3 and pages.dtype is torch.uint8 and stride[1:] == (shape[2], 1), "pages: uint8 layers of contiguous pages are wanted")
-    _want(pairs.size == 0 or (pairs.ndim == 2 and pairs.shape[1] == 2), "pairs: [n, 2] is wanted")
+    if not (len(shape) == 3 and pages.dtype is torch.uint8 and stride[1] == shape[2] and stride[2] == 1):
+        raise L.PM355Error("pages: uint8 layers of contiguous pages are wanted")
+    if pairs.size and (pairs.ndim != 2 or pairs.shape[1] != 2):
+        raise L.PM355Error("pairs: [n, 2] is wanted")
     if len(pairs):
         _kv4_call("pm355_pages_copy", pages.data_ptr(), shape[2], stride[0] if shape[0] > 1 else shape[1] * shape[2], shape[0], shape[1], pairs.ctypes.data, len(pairs),
                   torch._C._cuda_getCurrentRawStream(device))
