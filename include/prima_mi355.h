@@ -471,7 +471,8 @@ PM355_API size_t pm355_kv4_page_bytes(int n_head_kv, int head_dim);      /* 0: s
 /* Norm, rotation and cache store of new tokens in one launch (llm_build_norm on heads + ggml_rope_ext + llm_build_kv_store): per head y = x / sqrt(mean(x^2) + eps) * norm (with
  * `norm`; norm_q / norm_k f32 [head_dim] or NULL: no weight), then the first n_rot dimensions turn by pos * d_turns[i] turns, pairs (2 i, 2 i + 1) or, with rope_neox, (i, i + n_rot / 2),
  * times mscale. Queries go to q (type, rounded once), keys - formed in 64 bits, so that their codes depend on no order of sums - and values into the pages. A row with d_pos < 0, d_seq
- * outside [0, n_seq), or without a page at its position stores nothing in the cache (its query is written; position 0 is taken where d_pos < 0). Rows of one call have different (sequence, position). */
+ * outside [0, n_seq), or without a page at its position stores nothing in the cache (its query is written; position 0 is taken where d_pos < 0). Rows of one call have different (sequence, position). q may be the
+ * front of proj's own rows. */
 typedef struct {
     int32_t type, n_head, n_tokens;                             /* PM355_TYPE_BF16 or F32, of proj and q; n_head a multiple of n_head_kv */
     const void * proj; int64_t ld_proj;                         /* [n_tokens] rows [q: n_head d | k: n_head_kv d | v: n_head_kv d], ld_proj values apart (a multiple of 4, 16-byte aligned) */
@@ -490,8 +491,9 @@ PM355_API int pm355_rope_turns(const pm355_rope_params * rp, const float * freq_
  * weighted values; 0 for a query that sees nothing (position < 0 among them). Queries come in tiles of consecutive tokens of one sequence, device int32 {row, tokens, position of the first,
  * sequence} each, of at most tile_tokens tokens. n_head / n_head_kv * tile_tokens <= 16, or tile_tokens == 1: decoded and drafted tokens, keys split over workgroups by max_keys (the
  * most keys that a tile sees; only the speed depends on it); up to 128: prompts. Keys and values are the cache's f16 values; queries and probabilities are f16 with type BF16 (queries
- * scaled by a power of two per row) and pairs of f16 - 22 bits - with type F32; sums and softmax in f32. work: f32 scratch for split keys (>= pm355_attn_kv4_work_floats() lets every
- * split happen), zeroed once, left fit for the next call, used by one call at a time; NULL: no splits. Rows that no tile names are left as they are. */
+ * scaled by a power of two per row) and pairs of f16 - 22 bits - with type F32; sums and softmax in f32. work: f32 scratch for split keys, 16-byte aligned, of any size (pm355_attn_kv4_work_floats()
+ * lets every split happen) and with any contents, used by one call at a time - graphs captured with the same scratch do not run at once; NULL: no splits. Rows that no tile names are left as
+ * they are. */
 typedef struct {
     int32_t type, n_head; const void * q; int64_t ldq; void * out; int64_t ldo;      /* rows of n_head d values, ld a multiple of 8, 16-byte aligned */
     float scale; int32_t window, n_first;

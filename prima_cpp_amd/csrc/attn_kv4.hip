@@ -1,12 +1,15 @@
 // attn_kv4.hip — attention over pages held in 4 bits: causal, with a sliding window and first tokens that stay visible.
 //
 // o = sum_j p_j v_j / sum_j p_j, p_j = exp2(cf q k_j - max), over the j that the query sees; one pass over the keys with the running maximum and sum, both products on the f16 matrix cores.
-// Keys and values become f16 in registers: a pair of codes is masked out of a word over the bits of 1024, less 1032, times the scale - 3.25 operations for two values (the words are
+// Keys and values become f16 on their way to the products: a pair of codes is masked out of a word over the bits of 1024, less 1032, times the scale - 3.25 operations for two values (the words are
 // ordered so that a mask gives a pair that an operand wants). Queries are brought to [1, 2) by a power of two per row, exact for bf16; WIDE (32-bit rows) holds queries and probabilities as
 // pairs of f16 and makes two products of each. Probabilities are held times 2^8, so that f16 has its steps of 2^-11 down to p = 2^-22.
 // S^T = K Q^T is computed with the key rows permuted so that a lane's score registers are its P operand of O^T = V^T P^T.
-//   few    up to 16 columns (tokens x query heads of a KV head) per workgroup, 32 keys per wave and step straight from memory, keys split over waves and workgroups: bound by memory
-//   tiles  128 columns per workgroup, a page at a time through LDS, where it is made f16 once for all four waves: bound by the matrix cores and the vector work on scores
+//   few    16 or 32 columns (tokens x query heads of a KV head) per workgroup, 32 keys per wave and step, keys split over waves and workgroups: bound by memory. 48 tokens of 64 heads behind
+//          3300 .. 8203 keys 74 us (329 MB, 4.4 TB/s), one of 32 heads behind 131100 36 us (151 MB), 16 x 4 of 28 heads in a window of 4096 24 us; a large copy reaches 4.9 TB/s here
+//   tiles  128 columns per workgroup, a page at a time through LDS, where it is made f16 once for all four waves: bound by the matrix cores, which run at 1.1 .. 1.3 PFLOP/s under load.
+//          4096 tokens of 32 heads behind 2011: 316 us, 860 TFLOP/s (a large f16 product of the library 1110)
+//   join   the partial sums of split keys
 #include "pm355_kv4.h"
 #include "pm355_kernels.h"
 #include "../../include/prima_mi355.h"
@@ -151,7 +154,7 @@ template <typename T, int NB, bool WIDE, int CT> __global__ __launch_bounds__(FW
     constexpr int D = NB * 32, VT = D / 16, LD = D + 4, COLS = 16 * CT;
     typedef pm_kv4_slab<NB> S;
     typedef pm_step<NB> Q;
-    extern __shared__ __attribute__((aligned(16))) char lds[];            // [FW][STAGES] steps; then [FW][16][LD] sums; then what join() wants
+    extern __shared__ __attribute__((aligned(16))) char lds[];            // [FW][STAGES] steps; then [FW][16][LD] sums
     float * acc_l = (float *) lds;
     __shared__ float m_l[FW][16], l_l[FW][16];
     const uint32_t id = swizzled();
@@ -649,6 +652,9 @@ template <typename T, int D, int COLS> __global__ __launch_bounds__(256) void jo
     }
 }
 
+// FEW_WANT: one workgroup of 8 waves per CU is enough to fill the memory's queues, and every split costs its join. 32 tokens of 8 KV heads behind 8190 keys: 256 workgroups 67 us, 512 73, 1024 (of
+// 4 waves) 80; one token behind 262100: 72, 72, 82. FEW_COLS: up to there rows of keys are read again per 32 columns; 8 x 16 tokens x 4 heads behind 4000 34 us, as one tile of 128 columns 38.
+// TILES_WANT: 64 tokens behind 30000 58 us, with 256 61; 512 behind 8000 108 and 119. LEAST: pages that a split is worth (204 keys in 2 splits 10.5 us, in one 7.5).
 constexpr int FEW_WANT = 256, FEW_LEAST = 4, FEW_MOST = 128, FEW_COLS = 64, TILES_WANT = 512, TILES_LEAST = 8, TILES_MOST = 32;
 // workgroups over which the keys of a slot are split: as many as fill the chip, none with less than `least` pages, and what the scratch holds
 int splits_of(const pm_kv4_attn & a, int64_t slots, int64_t busy, int want, int least, int most, int64_t floats) {
@@ -672,11 +678,12 @@ template <typename T, int NB> int launch(const pm_kv4_cache & c, pm_kv4_attn a, 
     if (a.window > 0) { const int64_t most = (int64_t) a.window + a.tile_tokens + 128 + a.first; if (most < a.max_keys) a.max_keys = (int) most; }
     // columns of a tile on the average: tile_tokens only bounds them
     const int64_t cols = (int64_t) R * (a.n_tokens / a.n_tiles < a.tile_tokens ? (a.n_tokens + a.n_tiles - 1) / a.n_tiles : a.tile_tokens);
-    auto few = [&](auto kern, auto ctc) {
+    auto few = [&](auto kern, auto ctc) -> int {
         constexpr int ct = decltype(ctc)::value;
         const int passes = (R * a.tile_tokens + 16 * ct - 1) / (16 * ct), launched = ct > 1 ? (int) ((cols + 16 * ct - 1) / (16 * ct)) : passes;
         const int64_t slots = (int64_t) a.n_tiles * c.G * passes, busy = (int64_t) a.n_tiles * c.G * launched;
         const int splits = splits_of(a, slots, busy, FEW_WANT, FEW_LEAST, FEW_MOST, 16 * ct * (D + 2));
+        if (busy * splits >= 1 << 23 || slots >= 1 << 20) return PM355_E_SHAPE;      // (a launch has fewer than 2^32 threads, that of the joins up to 16 workgroups of 256 per slot)
         const size_t ring = (size_t) FW * STAGES * pm_step<NB>::BYTES, acc = (size_t) FW * 16 * (D + 4) * 4, lds = ring > acc ? ring : acc;
         pm_allow_big_lds((const void *) kern, lds);
         hipLaunchKernelGGL(kern, dim3((unsigned) (busy * splits)), dim3(FW * 64), lds, st, c, a, launched, passes, splits);
@@ -690,6 +697,7 @@ template <typename T, int NB> int launch(const pm_kv4_cache & c, pm_kv4_attn a, 
     const int64_t slots = (int64_t) a.n_tiles * c.G;
     const int splits = splits_of(a, slots, slots, TILES_WANT, TILES_LEAST, TILES_MOST, TC * (D + 2));
     const size_t lds = 2 * ((size_t) PM_PAGE * (D * 2 + 16) + D * (PM_PAGE * 2 + 16));
+    if (slots * splits >= 1 << 24 || (splits > 1 && slots >= 1 << 17)) return PM355_E_SHAPE;
     static_assert(2 * (PM_PAGE * (D * 2 + 16) + D * (PM_PAGE * 2 + 16)) >= TC * (D + 4) * 4, "the partial sums go through the pages' LDS");
     pm_allow_big_lds((const void *) tiles_kernel<T, NB, WIDE>, lds);
     hipLaunchKernelGGL((tiles_kernel<T, NB, WIDE>), dim3((unsigned) slots, splits), dim3(256), lds, st, c, a, splits);

@@ -227,7 +227,7 @@ int pm_launch_kv4_append(const pm_kv4_cache & c, const pm_kv4_append & a, hipStr
     const int rpw = c.d <= 64 ? 8 : c.d <= 128 ? 4 : 2, groups = 2 * ((c.G + rpw - 1) / rpw) + (a.H + rpw - 1) / rpw, fill = 8192 / a.T;
     const int parts = fill < 1 ? 1 : fill < groups ? fill : groups;
     const int64_t blocks = ((int64_t) a.T * parts + 3) / 4;
-    if (blocks > 0x3fffffff) return PM355_E_SHAPE;
+    if (blocks >= 1 << 24) return PM355_E_SHAPE;           // (a launch has fewer than 2^32 threads)
 #define PM_CALL(NB) \
     if (a.type == PM_BF16) hipLaunchKernelGGL((append_kernel<uint16_t, NB>), dim3((unsigned) blocks), dim3(256), 0, st, c, a, parts); \
     else hipLaunchKernelGGL((append_kernel<float, NB>), dim3((unsigned) blocks), dim3(256), 0, st, c, a, parts)

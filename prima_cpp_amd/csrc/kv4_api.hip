@@ -33,7 +33,7 @@ int pm355_kv4_append(const pm355_kv4_cache * c, const pm355_kv4_append_args * p,
     if (!p || !known(p->type)) return fail(PM355_E_UNSUPPORTED, "kv4_append: type");
     if (p->n_tokens == 0) return 0;
     if (p->n_tokens < 0 || p->n_head < 1 || p->n_head % c->n_head_kv || !p->proj || !p->q || !p->d_pos || !p->d_seq || p->ld_proj < ((int64_t) p->n_head + 2 * c->n_head_kv) * d ||
-        p->ldq < (int64_t) p->n_head * d || (int64_t) p->n_head * d > 0x3fffffff)
+        p->ldq < (int64_t) p->n_head * d || (int64_t) p->n_head * d > 0x0fffffff)
         return fail(PM355_E_SHAPE, "kv4_append: shape");
     if (p->d_turns && (p->n_rot < 8 || p->n_rot % 8 || p->n_rot > d)) return fail(PM355_E_SHAPE, "kv4_append: n_rot");
     if (p->ld_proj % 4 || p->ldq % 4 || !aligned(p->proj, 16) || !aligned(p->q, 16)) return fail(PM355_E_ALIGN, "kv4_append: rows");
@@ -73,7 +73,7 @@ int pm355_attn_kv4(const pm355_kv4_cache * c, const pm355_attn_kv4_args * p, pm3
     const int64_t d = c->head_dim;
     if (!p || !known(p->type)) return fail(PM355_E_UNSUPPORTED, "attn_kv4: type");
     if (p->n_tiles == 0) return 0;
-    if (p->n_tiles < 0 || p->n_tokens < 1 || p->n_head < 1 || p->n_head % c->n_head_kv || !p->q || !p->out || !p->d_tiles || p->ldq < p->n_head * d || p->ldo < p->n_head * d || p->n_head * d > 0x3fffffff ||
+    if (p->n_tiles < 0 || p->n_tokens < 1 || p->n_head < 1 || p->n_head % c->n_head_kv || !p->q || !p->out || !p->d_tiles || p->ldq < p->n_head * d || p->ldo < p->n_head * d || p->n_head * d > 0x0fffffff ||
         p->window < 0 || p->n_first < 0 || p->max_keys < 0)
         return fail(PM355_E_SHAPE, "attn_kv4: shape");
     if (p->tile_tokens < 1 || (p->tile_tokens > 1 && (int64_t) p->n_head / c->n_head_kv * p->tile_tokens > 128)) return fail(PM355_E_SHAPE, "attn_kv4: tile_tokens");
@@ -86,7 +86,7 @@ int pm355_attn_kv4(const pm355_kv4_cache * c, const pm355_attn_kv4_args * p, pm3
 
 int pm355_pages_copy(void * pages, size_t page_bytes, size_t layer_bytes, int n_layers, int n_pages, const int32_t * pairs, int n_pairs, pm355_stream_t st) {
     if (n_pairs == 0) return 0;
-    if (!pages || !pairs || n_pairs < 0 || n_layers < 1 || n_pages < 1 || page_bytes < 16 || page_bytes > (size_t) 1 << 40 || (n_layers > 1 && layer_bytes / page_bytes < (size_t) n_pages))
+    if (!pages || !pairs || n_pairs < 0 || n_layers < 1 || n_pages < 1 || page_bytes < 16 || page_bytes > (size_t) 1 << 32 || (n_layers > 1 && layer_bytes / page_bytes < (size_t) n_pages))
         return fail(PM355_E_SHAPE, "pages_copy: shape");
     if (page_bytes % 16 || layer_bytes % 16 || !aligned(pages, 16)) return fail(PM355_E_ALIGN, "pages_copy: pages");
     try {

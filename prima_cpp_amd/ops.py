@@ -706,7 +706,8 @@ def rope_turns(n_dims, n_ctx_orig=8192, freq_base=10000.0, freq_scale=1.0, ext_f
 
 def kv4_append(proj, pages, table, pos, seq, n_head, n_head_kv, head_dim, q=None, norm=False, norm_q=None, norm_k=None, eps=1e-6, turns=None, mscale=1.0, neox=False):
     """Queries normed and rotated (returned, [T, n_head * head_dim] in the type of proj), keys likewise and values into 4-bit pages. proj [T, >= (n_head + 2 n_head_kv) * head_dim] rows
-    q | k | v, f32 or bf16; pages uint8 [n, kv4_page_bytes()], table int32 [sequences, pages of a sequence], pos, seq int32 [T]; turns (rope_turns): None rotates nothing."""
+    q | k | v, f32 or bf16; pages uint8 [n, kv4_page_bytes()], table int32 [sequences, pages of a sequence], pos, seq int32 [T]; turns (rope_turns): None rotates nothing. q: where the queries
+    go, also proj's own front. A row with a negative position, an unknown sequence or no page at its position stores nothing."""
     device = _same_device(proj, pages, table, pos, seq, q, norm_q, norm_k, turns)
     c, ty, T, dtype, width = _kv4_cache(pages, table, n_head_kv, head_dim), _act("proj", proj), proj.shape[0], proj.dtype, n_head * head_dim
     at, ld = _rows("proj", proj, T, width + 2 * n_head_kv * head_dim, 4)
@@ -757,14 +758,16 @@ def kv4_tiles(entries, n_head, n_head_kv):
 
 
 def kv4_work(n_head, n_head_kv, head_dim):
-    """scratch that lets attn_kv4 split the keys of few rows over workgroups: zeroed here, for one call at a time"""
+    """scratch that lets attn_kv4 split the keys of few rows over workgroups, for one call at a time"""
     n = L.declare("pm355_attn_kv4_work_floats", _sz, [_i32, _i32, _i32])(n_head, n_head_kv, head_dim)
-    return torch.zeros(n, device=_dev())
+    if not n:
+        raise L.PM355Error("%d heads over %d KV heads of %d are not supported" % (n_head, n_head_kv, head_dim))
+    return torch.empty(n, device=_dev())
 
 
 def attn_kv4(q, pages, table, tiles, tile_tokens, max_keys, n_head, n_head_kv, head_dim, scale, window=0, n_first=0, out=None, work=None):
     """Attention of q [T, n_head * head_dim] (f32 or bf16) over 4-bit pages: causal, with window > 0 only the last `window` keys and the first n_first. tiles int32 [n, 4] {row, tokens,
-    position, sequence} (kv4_tiles). Returns out, of which the rows that tiles name are written. work: kv4_work(), for one call at a time."""
+    position, sequence} (kv4_tiles). Returns out, of which the rows that tiles name are written. work: kv4_work(), for one call at a time; None splits no keys."""
     device = _same_device(q, pages, table, tiles, out, work)
     c, ty, dtype, T, of, width = _kv4_cache(pages, table, n_head_kv, head_dim), _act("q", q), q.dtype, q.shape[0], tiles.shape, n_head * head_dim
     q_at, ldq = _rows("q", q, T, width, 8)
@@ -791,7 +794,12 @@ def attn_kv4(q, pages, table, tiles, tile_tokens, max_keys, n_head, n_head_kv, h
 def pages_copy(pages, pairs):
     """pages[.., to] = pages[.., from] for (from, to) pairs on the host: uint8 [layers, n, page bytes] or [n, page bytes]; every `to` stands once and is no `from`"""
     device = _same_device(pages)
-    pairs = np.ascontiguousarray(pairs, np.int32)
+    pairs = np.asarray(pairs)
+    if pairs.dtype != np.int32:
+        if pairs.size and (pairs.dtype.kind not in "iu" or pairs.min() < 0 or pairs.max() > 0x7fffffff):
+            raise L.PM355Error("pairs: page numbers are wanted")
+        pairs = pairs.astype(np.int32)
+    pairs = np.ascontiguousarray(pairs)
     shape, stride = pages.shape, pages.stride()
     if len(shape) == 2:
         shape, stride = (1, *shape), (0, *stride)

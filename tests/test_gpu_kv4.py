@@ -125,6 +125,21 @@ def test_append_rows_without_a_place():
 
 
 @pytest.mark.parametrize("type", ["bf16", "f32"])
+@pytest.mark.parametrize("T", [1, 70])
+def test_append_in_place(T, type):
+    """queries over the front of their own projections"""
+    G, H, d = 2, 12, 128
+    proj = torch.randn(T, (H + 2 * G) * d, device="cuda").to(TYPES[type])
+    table, turns = torch.arange(2, dtype=torch.int32, device="cuda")[None], ops.rope_turns(d)[0]
+    pos, seq = torch.arange(T, dtype=torch.int32, device="cuda"), torch.zeros(T, dtype=torch.int32, device="cuda")
+    a, b = (torch.zeros(2, ops.kv4_page_bytes(G, d), dtype=torch.uint8, device="cuda") for _ in range(2))
+    q = ops.kv4_append(proj, a, table, pos, seq, H, G, d, norm=True, turns=turns, neox=True)
+    x = proj.clone()
+    ops.kv4_append(x, b, table, pos, seq, H, G, d, q=x[:, :H * d], norm=True, turns=turns, neox=True)
+    assert torch.equal(x[:, :H * d], q) and torch.equal(x[:, H * d:], proj[:, H * d:]) and torch.equal(a, b)
+
+
+@pytest.mark.parametrize("type", ["bf16", "f32"])
 def test_append_borders(type):
     """zeros, both signs of the largest value, ties between codes, values that a 16-bit scale cannot hold, NaN and infinities"""
     G, H, d = 1, 1, 64
@@ -153,7 +168,7 @@ def test_append_borders(type):
 
 
 # ---- attention --------------------------------------------------------------------------------------------------------------
-def attend_case(d, H, G, type, entries, window=0, first=0, seed=0, drop=(), spread=0.1, work=True, break_pages=None, gain=1.0, stride=0):
+def attend_case(d, H, G, type, entries, window=0, first=0, seed=0, drop=(), spread=0.1, work=True, break_pages=None, gain=1.0, stride=0, scale=None):
     """entries (sequence, first new position, new tokens); compares every row with the restatement, returns the output"""
     r = np.random.default_rng(seed)
     n_seq = max(s for s, _, _ in entries) + 1
@@ -169,7 +184,7 @@ def attend_case(d, H, G, type, entries, window=0, first=0, seed=0, drop=(), spre
     tiles, tile, keys = ops.kv4_tiles(entries, H, G)
     out = torch.full((T + 1, H * d + stride), 5.0, dtype=TYPES[type], device="cuda")
     qd = torch.cat([q, q[:1]]).cuda()
-    scale = d ** -0.5
+    scale = d ** -0.5 if scale is None else scale
     w = ops.kv4_work(H, G, d) if work else None
     ops.attn_kv4(qd[:, :H * d], dev(raw), dev(table), dev(tiles), tile, keys, H, G, d, scale, window, first, out=out[:, :H * d], work=w)
     if work:                                                # a second call on the same scratch
@@ -314,6 +329,22 @@ def test_attend_split_keys(entries, type):
     attend_case(128, 8, 2, type, entries, gain=2.0, window=2500, first=70)
 
 
+@pytest.mark.parametrize("type", ["bf16", "f32"])
+@pytest.mark.parametrize("d", [64, 128, 192])
+@pytest.mark.parametrize("entries", [[(0, 700, 18)] + [(s, 40 * s, 1) for s in range(1, 12)], [(0, 130, 17), (1, 0, 3), (2, 64, 2), (3, 900, 4), (4, 63, 5)]])
+def test_attend_unequal_tiles(entries, d, type):
+    """tiles whose columns are many more than those of the others, for which the launch is made"""
+    attend_case(d, 14, 2, type, entries)
+    attend_case(d, 14, 2, type, entries, window=90, first=5)
+
+
+@pytest.mark.parametrize("type", ["bf16", "f32"])
+@pytest.mark.parametrize("scale", [-0.08, 0.0, 3.0])
+@pytest.mark.parametrize("n", [1, 40])
+def test_attend_scales(n, scale, type):
+    attend_case(128, 8, 2, type, [(0, 333, n), (1, 64, n)], scale=scale)
+
+
 def test_attend_rows_nobody_names():
     """tiles of padded rows: position < 0 gives zeros, rows outside the tensors and empty tiles nothing"""
     r = np.random.default_rng(0)
@@ -393,7 +424,7 @@ def test_refusals():
                 dict(n_first=-1), dict(out=q.bfloat16()), dict(out=q[:2]), dict(work=z(4, t=torch.float64)), dict(max_keys=-1), dict(n_head=5)):
         with pytest.raises(L.PM355Error):
             ops.attn_kv4(**{**good, **bad})
-    for bad in ([(0, 2)], [(0, 0)], [(-1, 0)], [(0, 1), (1, 0)]):
+    for bad in ([(0, 2)], [(0, 0)], [(-1, 0)], [(0, 1), (1, 0)], [(0, 1 << 32)], [(0.0, 1.0)], [0, 1]):
         with pytest.raises(L.PM355Error):
             ops.pages_copy(pages, bad)
     with pytest.raises(L.PM355Error):
