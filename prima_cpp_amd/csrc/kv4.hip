@@ -1,7 +1,8 @@
 // kv4.hip — into a 4-bit KV cache and out of it: per-head norm of queries and keys, rotation, rounding to 4 bits, one pass over the projections.
 //
 // y = x / sqrt(mean(x^2) + eps) w;  (a, b) -> (a cos - b sin, b cos + a sin) mscale at 2 pi frac(pos turns_i);  scale = f16(M / -8), code = clamp(rint(y / scale), -8, 7) + 8.
-// Bound by memory: a row of (H + 2 G) d values is read once, H d values and 1.125 G d bytes are written.
+// Bound by memory: a row of (H + 2 G) d values is read once, H d values and 1.125 G d bytes are written. 6001 tokens of 32 + 8 heads of 128 (bf16, norm, rotation) 36 us for 130 MB, without keys and
+// values 24 for 98 MB (the scattered bytes of the values are 4 us of the difference); 48 tokens of 64 + 8 heads 5.2 us, one token 4.0. Reading 6001 tokens back 9.7 us (31 MB).
 #include "pm355_kv4.h"
 #include "pm355_kernels.h"
 #include "../../include/prima_mi355.h"
