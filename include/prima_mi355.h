@@ -492,8 +492,8 @@ PM355_API int pm355_rope_turns(const pm355_rope_params * rp, const float * freq_
  * sequence} each, of at most tile_tokens tokens. n_head / n_head_kv * tile_tokens <= 16, or tile_tokens == 1: decoded and drafted tokens, keys split over workgroups by max_keys (the
  * most keys that a tile sees; only the speed depends on it); up to 128: prompts. Keys and values are the cache's f16 values; queries and probabilities are f16 with type BF16 (queries
  * scaled by a power of two per row) and pairs of f16 - 22 bits - with type F32; sums and softmax in f32. work: f32 scratch for split keys, 16-byte aligned, of any size (pm355_attn_kv4_work_floats()
- * lets every split happen) and with any contents, used by one call at a time - graphs captured with the same scratch do not run at once; NULL: no splits. Rows that no tile names are left as
- * they are. */
+ * lets every split happen) and with any contents, used by one call at a time - graphs captured with the same scratch do not run at once; NULL: no splits. out may be q. Rows that no tile
+ * names are left as they are. */
 typedef struct {
     int32_t type, n_head; const void * q; int64_t ldq; void * out; int64_t ldo;      /* rows of n_head d values, ld a multiple of 8, 16-byte aligned */
     float scale; int32_t window, n_first;

@@ -177,8 +177,8 @@ template <typename T, int NB, bool WIDE, int CT> __global__ __launch_bounds__(FW
     const char * head = c.pages + (size_t) g * S::BYTES;
     auto page_of = [&](int i) __attribute__((always_inline)) { if (!known || i >= end) return -1; const int p = table[page_at(see, i >> 1)]; return (unsigned) p < (unsigned) c.n_pages ? p : -1; };
     const uint32_t krow = 8 * (lr >> 2) + (lr & 3);        // key of score row lr in the first 16 of a step (the second: + 4)
-    // Codes go from memory to LDS in whole lines and from there to the lanes that want them: straight to registers a quarter of a wave's lanes would each want 16 bytes of another line of 64,
-    // four times the lines a load can ask for per cycle. Rows whose pieces would meet in a bank are turned against each other.
+    // Codes go from memory to LDS in whole lines and from there to the lanes that want them (straight to registers every lane wants 16 bytes of another line of 64, and a step on its way costs
+    // 36 registers: no slower with 4 waves of 128 registers, but 8 of them do not fit). Rows whose pieces would meet in a bank are turned against each other.
     constexpr int TURN = NB % 4 ? 0 : NB / 4;
     char * const ring = lds + wave * STAGES * Q::BYTES;
     const uint32_t ring_at = (uint32_t) (uintptr_t) (__attribute__((address_space(3))) char *) lds + wave * STAGES * Q::BYTES;

@@ -359,6 +359,24 @@ def test_attend_rows_nobody_names():
         assert (o[[1, 4]] == 5.0).all() and not o[[2, 3]].any() and (o[[0, 5]] != 5.0).all()
 
 
+@pytest.mark.parametrize("n", [1, 60])
+@pytest.mark.parametrize("floats", [0, 64, 70_000, 1_000_000])
+def test_scratch_of_any_size_and_contents(floats, n):
+    """and the output over the queries"""
+    H, G, d = 8, 2, 128
+    r = np.random.default_rng(0)
+    table, pages = tables([9000 + n, 70 + n], r)
+    pages, table = dev(random_pages(pages, G, d, r)), dev(table)
+    tiles, tile, keys = ops.kv4_tiles([(0, 9000, n), (1, 70, n)], H, G)
+    q = torch.randn(2 * n, H * d, device="cuda")
+    args = (pages, table, dev(tiles), tile, keys, H, G, d, 0.1)
+    want = ops.attn_kv4(q, *args)
+    work = torch.full((floats,), float("nan"), device="cuda")
+    assert torch.allclose(ops.attn_kv4(q, *args, work=work), want, rtol=1e-5, atol=1e-5)
+    x = q.clone()
+    assert torch.equal(ops.attn_kv4(x, *args, out=x, work=work), ops.attn_kv4(q, *args, work=work)) and x.data_ptr() != q.data_ptr()
+
+
 def test_far_offsets():
     """a pool beyond 4 GB, a position beyond 2^20"""
     H, G, d, n = 8, 8, 128, 60000
