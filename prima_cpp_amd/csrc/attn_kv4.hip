@@ -474,10 +474,10 @@ template <typename T, int NB, bool WIDE> __global__ __launch_bounds__(256, NB <=
     // Two pages in LDS: while the scores of one are formed on the matrix cores, the vector pipe makes the next one f16; the products with the values run among the exponentials
     for (int i = begin, stage = 0; i < end; ++i, stage ^= 1) {
         const int after = page_of(i + 2), key0 = page_at(see, i) * PM_PAGE;
-        const bool all = whole(i, page), there = page >= 0;
-        if (i + 1 < end && !whole(i + 1, next)) { asm volatile(""); clean(stage ^ 1); }
+        const bool all = whole(i, page), there = page >= 0, dirty = i + 1 < end && !whole(i + 1, next);
         page = next; next = after;
-        __syncthreads();                                   // (this page is there, the other stage is read)
+        __syncthreads();                                   // (this page is there, the other stage and its flags are read)
+        if (dirty) { asm volatile(""); clean(stage ^ 1); }
         const char * k_l = lds + stage * STAGE, * v_l = k_l + PM_PAGE * KL;
         f32x16 sc[2];
 #pragma unroll

@@ -290,6 +290,23 @@ def test_attend_garbage_in_masked_places(n, type):
 
 
 @pytest.mark.parametrize("type", ["bf16", "f32"])
+@pytest.mark.parametrize("d", [64, 128])
+def test_attend_garbage_two_pages_on(d, type):
+    """tiles over three pages, none of which all of their queries see: what the last one's hidden slots hold is no matter of the first one's keys"""
+    s, heads, entries = P.slab(d), 4, [(i, 40, 90) for i in range(24)]
+
+    def spoil(pages, table):
+        b = pages.reshape(len(pages), heads, s["bytes"])
+        for part, order in (("ks", (64, -1)), ("vs", (-1, 64))):
+            x = b[..., s[part]:s[part] + 128 * (d // 32)].view(np.float16).reshape(len(pages), heads, *order)
+            x = x if part == "ks" else x.swapaxes(2, 3)
+            x[table[:, 2], :, 2:] = np.nan
+
+    out = attend_case(d, heads, heads, type, entries, break_pages=spoil)
+    assert torch.isfinite(out).all()
+
+
+@pytest.mark.parametrize("type", ["bf16", "f32"])
 @pytest.mark.parametrize("where", ["key", "value"])
 @pytest.mark.parametrize("n", [3, 80])
 def test_attend_nan_reaches_those_who_see_it(n, where, type):
