@@ -24,7 +24,8 @@ typedef uint32_t u32x3 __attribute__((ext_vector_type(3), aligned(4)));
 typedef uint16_t u16x4 __attribute__((ext_vector_type(4)));
 
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr float NONE = -1e30f;                             // running maximum before the first visible key
+constexpr float NONE = -3e38f;                             // running maximum before the first visible key
+constexpr float FAR = 16777216.0f;                         // beyond 2^24 a maximum is rounded by more than 1 (2^15 is the last power that f16 has): scores are rounded like it, then it is taken off
 constexpr float HELD = 8.0f, SLACK = 6.0f;                 // probabilities are held times 2^HELD; the running maximum may lag by SLACK (2^14 < 65504), sums are seldom rescaled
 
 // N words (N halves) that lie side by side, a multiple of 4 N (2 N) bytes into a slab
@@ -89,11 +90,11 @@ __device__ __forceinline__ void split_f16(const float * x, f16x8 & hi, f16x8 & l
 #pragma unroll
     for (int j = 0; j < 8; ++j) { hi[j] = (_Float16) x[j]; lo[j] = (_Float16) (x[j] - (float) hi[j]); }
 }
-// 2^-e with the sign of scale for a row whose largest magnitude is in [2^e, 2^(e + 1)); cf = |scale| log2(e) 2^e
+// 2^-e with the sign of scale for a row whose largest magnitude is in [2^e, 2^(e + 1)); cf = |scale| log2(e) 2^e, up to 2^100: scores (below 2^25) differ by 2^-48 at the least
 __device__ __forceinline__ float row_factor(float most, float scale, float & cf) {
     int e = (int) (__builtin_bit_cast(uint32_t, most) >> 23 & 255) - 127;
-    e = e < -100 ? -100 : e > 100 ? 0 : e;                 // (a row of zeros; rows that are not finite stay so)
-    cf = fmaxf(fabsf(scale) * LOG2E * ldexpf(1.0f, e), 1e-30f);
+    e = e < -100 ? -100 : e > 127 ? 0 : e;                 // (a row of zeros; rows that are not finite stay so)
+    cf = fminf(fmaxf(fabsf(scale) * LOG2E * ldexpf(1.0f, e), 1e-30f), 0x1p100f);
     return copysignf(ldexpf(1.0f, -e), scale);
 }
 
@@ -207,6 +208,7 @@ template <typename T, int NB, bool WIDE, int CT> __global__ __launch_bounds__(FW
     f32x4 acc[CT][VT];
     float cf[CT], m[CT], l[CT];
     int pos[CT];
+    bool far = false;
 #pragma unroll
     for (int u = 0; u < CT; ++u) {
         const int col = u * 16 + lr, tok = (col0 + col) / R, row = row0 + tok, h = g * R + (col0 + col) % R;
@@ -298,14 +300,21 @@ template <typename T, int NB, bool WIDE, int CT> __global__ __launch_bounds__(FW
             if (__any(mx > m[u] + SLACK)) {
                 const float mn = fmaxf(m[u], mx), corr = __builtin_amdgcn_exp2f(m[u] - mn);
                 m[u] = mn; l[u] *= corr;
+                far |= __any(fabsf(mn) > FAR && mn > NONE);
 #pragma unroll
                 for (int t = 0; t < VT; ++t)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) acc[u][t][e] *= corr;
             }
-            const float mo = HELD - m[u];
+            float k = cf[u], mo = HELD - m[u];
+            if (far) {
+                asm volatile("");
 #pragma unroll
-            for (int j = 0; j < 8; ++j) { f[j] = __builtin_amdgcn_exp2f(fmaf(f[j], cf[u], mo)); l[u] += f[j]; }
+                for (int j = 0; j < 8; ++j) f[j] = f[j] * k - m[u];
+                k = 1.0f; mo = HELD;
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) { f[j] = __builtin_amdgcn_exp2f(fmaf(f[j], k, mo)); l[u] += f[j]; }
             split_f16(f, ph[u], pl[u]);
         }
 #pragma unroll
@@ -465,6 +474,7 @@ template <typename T, int NB, bool WIDE> __global__ __launch_bounds__(256, NB <=
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[t][e] = 0.0f;
     float m = NONE, l = 0.0f;
+    bool far = false;
     const int krow = (lr & 0x13) | (lr >> 3 & 1) << 2 | (lr >> 2 & 1) << 3;       // key of score row lr: bits 2 and 3 changed over
     if (begin < end) {
         if (!whole(begin, page)) { asm volatile(""); clean(0); }
@@ -523,15 +533,24 @@ template <typename T, int NB, bool WIDE> __global__ __launch_bounds__(256, NB <=
         if (__any(mx > m + SLACK)) {
             const float mn = fmaxf(m, mx), corr = __builtin_amdgcn_exp2f(m - mn);
             m = mn; l *= corr;
+            far |= __any(fabsf(mn) > FAR && mn > NONE);
 #pragma unroll
             for (int t = 0; t < VT; ++t)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) acc[t][e] *= corr;
         }
-        const float mo = HELD - m;
+        float k = cf, mo = HELD - m;
+        if (far) {
+            asm volatile("");
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) sc[t][e] = sc[t][e] * k - m;
+            k = 1.0f; mo = HELD;
+        }
         f16x2 ph[2][4], pl[2][4];                          // probabilities of 16 keys, and of the next 16
         auto weigh = [&](int j, int e) __attribute__((always_inline)) {
-            const float p = __builtin_amdgcn_exp2f(fmaf(sc[j >> 1][(j & 1) * 8 + 2 * e], cf, mo)), q = __builtin_amdgcn_exp2f(fmaf(sc[j >> 1][(j & 1) * 8 + 2 * e + 1], cf, mo));
+            const float p = __builtin_amdgcn_exp2f(fmaf(sc[j >> 1][(j & 1) * 8 + 2 * e], k, mo)), q = __builtin_amdgcn_exp2f(fmaf(sc[j >> 1][(j & 1) * 8 + 2 * e + 1], k, mo));
             l += p; l += q;
             const f16x2 h = {(_Float16) p, (_Float16) q};
             ph[j & 1][e] = h;

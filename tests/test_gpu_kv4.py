@@ -334,6 +334,39 @@ def test_attend_ranges(gain, spread, type):
 
 
 @pytest.mark.parametrize("type", ["bf16", "f32"])
+@pytest.mark.parametrize("entries", [[(0, 333, 1), (1, 64, 1)], [(0, 9000, 1)], [(0, 300, 7), (1, 64, 7)], [(0, 333, 33)], [(0, 9000, 40)]])
+@pytest.mark.parametrize("gain", [1e6, 1e9, 1e18, 1e31, 1e37])
+def test_attend_far_scores(gain, entries, type):
+    """scores up to the largest that a query of its type can make: the value of the key with the largest one, whose probability (1, or any number of f16 steps over the sum of just that)
+    is rounded once in the probabilities and once in the output. Rows whose two largest scores lie nearer to each other than the score sums' error are not compared."""
+    H, G, d, r = 8, 2, 128, np.random.default_rng(len(entries))
+    table, n = tables([p + m for _, p, m in entries], r)
+    raw = random_pages(n, G, d, r)
+    tiles, tile, keys = ops.kv4_tiles(entries, H, G)
+    q = torch.from_numpy((gain * r.normal(size=(sum(m for *_, m in entries), H * d))).astype(np.float32)).to(TYPES[type])
+    for scale in (0.088, -1.0):
+        got = ops.attn_kv4(q.cuda(), dev(raw), dev(table), dev(tiles), tile, keys, H, G, d, scale, work=ops.kv4_work(H, G, d)).double().cpu().numpy()
+        k, v = P.unpack(raw, G, d)
+        row, compared, half = 0, 0, torch.finfo(TYPES[type]).eps / 2
+        for s, p0, m in entries:
+            held = (p0 + m + 63) // 64
+            ks, vs = (z[table[s, :held]].transpose(1, 0, 2, 3).reshape(G, -1, d).astype(np.float64) for z in (k, v))
+            for i in range(m):
+                for h in range(H):
+                    x = q[row + i, h * d:(h + 1) * d].double().numpy()
+                    score = ks[h * G // H][:p0 + i + 1] @ x * scale
+                    at = np.argsort(score)[-2:]
+                    B = (np.abs(ks[h * G // H]) @ np.abs(x)).max() * abs(scale)
+                    if score[at[1]] - score[at[0]] < max(40.0, 4 * (d + 2) * 2.0 ** -24 * B):
+                        continue
+                    want = vs[h * G // H][at[1]]
+                    assert (np.abs(got[row + i, h * d:(h + 1) * d] - want) <= (half + 2.0 ** -11 + 2.0 ** -18) * np.abs(want)).all(), (s, i, h)
+                    compared += 1
+            row += m
+        assert compared > row * H // 2
+
+
+@pytest.mark.parametrize("type", ["bf16", "f32"])
 def test_attend_strides_and_no_scratch(type):
     attend_case(128, 8, 2, type, [(0, 1000, 1), (1, 3, 1)], stride=24, work=False)
     attend_case(128, 8, 2, type, [(0, 1000, 50), (1, 3, 1)], stride=8, work=False)
