@@ -86,7 +86,7 @@ int pm355_attn_kv4(const pm355_kv4_cache * c, const pm355_attn_kv4_args * p, pm3
 
 int pm355_pages_copy(void * pages, size_t page_bytes, size_t layer_bytes, int n_layers, int n_pages, const int32_t * pairs, int n_pairs, pm355_stream_t st) {
     if (n_pairs == 0) return 0;
-    if (!pages || !pairs || n_pairs < 0 || n_layers < 1 || n_pages < 1 || page_bytes < 16 || page_bytes > (size_t) 1 << 32 || (n_layers > 1 && layer_bytes / page_bytes < (size_t) n_pages))
+    if (!pages || !pairs || n_pairs < 0 || n_pairs > n_pages || n_pages > 0x3fffffff || n_layers < 1 || n_pages < 1 || page_bytes < 16 || page_bytes > (size_t) 1 << 32 || (n_layers > 1 && layer_bytes / page_bytes < (size_t) n_pages))
         return fail(PM355_E_SHAPE, "pages_copy: shape");
     if (page_bytes % 16 || layer_bytes % 16 || !aligned(pages, 16)) return fail(PM355_E_ALIGN, "pages_copy: pages");
     try {

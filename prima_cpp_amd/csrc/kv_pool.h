@@ -39,6 +39,8 @@ struct pm355_page_pool {
         const int n = missing(s, n_tokens);
         if (n > max_seq_pages - seqs[s].hi) return PM355_E_RANGE;
         if (n > (int) free_list.size()) return PM355_E_NOMEM;
+        room((size_t) n);
+        seqs[s].page.reserve(seqs[s].page.size() + n);
         for (int i = 0; i < n; ++i) {
             seqs[s].page.push_back(free_list.back());
             free_list.pop_back();

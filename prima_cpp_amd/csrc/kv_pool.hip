@@ -7,12 +7,12 @@ template <class F> static int guarded(F && f) { try { return f(); } catch (...) 
 
 extern "C" {
 pm355_page_pool * pm355_page_pool_new(int n_pages, int n_seqs, int max_seq_pages) {
-    return n_pages > 0 && n_seqs > 0 && max_seq_pages > 0 ? new pm355_page_pool(n_pages, n_seqs, max_seq_pages) : nullptr;
+    try { return n_pages > 0 && n_seqs > 0 && max_seq_pages > 0 ? new pm355_page_pool(n_pages, n_seqs, max_seq_pages) : nullptr; } catch (...) { return nullptr; }
 }
 void pm355_page_pool_free(pm355_page_pool * p) { delete p; }
 int pm355_page_pool_open(pm355_page_pool * p) { return p->open(); }
 int pm355_page_pool_close(pm355_page_pool * p, int seq) { return p->close(seq); }
-int pm355_page_pool_grow(pm355_page_pool * p, int seq, int n_tokens) { return p->grow(seq, n_tokens); }
+int pm355_page_pool_grow(pm355_page_pool * p, int seq, int n_tokens) { return guarded([&] { return p->grow(seq, n_tokens); }); }
 int pm355_page_pool_drop_before(pm355_page_pool * p, int seq, int position) { return p->drop_before(seq, position); }
 int pm355_page_pool_drop(pm355_page_pool * p, int seq, int from, int to) { return p ? p->drop(seq, from, to) : PM355_E_RANGE; }
 int pm355_page_pool_fork(pm355_page_pool * p, int seq, int n_tokens) { return p ? guarded([&] { return p->fork(seq, n_tokens); }) : PM355_E_RANGE; }

@@ -730,7 +730,11 @@ def kv4_append(proj, pages, table, pos, seq, n_head, n_head_kv, head_dim, q=None
         t_at, n_rot = turns.data_ptr(), 2 * turns.shape[0]
     pos, seq = _per_token("pos", pos, T), _per_token("seq", seq, T)
     if T:
-        _kv4_call("pm355_kv4_append", c, _KV4_APPEND.pack(ty, n_head, T, at, ld, q_at, ldq, norm, w_q, w_k, eps, t_at, n_rot, neox, mscale, pos, seq), torch._C._cuda_getCurrentRawStream(device))
+        try:
+            args = _KV4_APPEND.pack(ty, n_head, T, at, ld, q_at, ldq, norm, w_q, w_k, eps, t_at, n_rot, neox, mscale, pos, seq)
+        except (struct.error, OverflowError) as e:
+            raise L.PM355Error("kv4_append: %s" % e) from None
+        _kv4_call("pm355_kv4_append", c, args, torch._C._cuda_getCurrentRawStream(device))
     return q
 
 
@@ -786,8 +790,11 @@ def attn_kv4(q, pages, table, tiles, tile_tokens, max_keys, n_head, n_head_kv, h
     else:
         out_at, ldo = _rows("out", out, T, width, 8)
     if T and of[0]:
-        _kv4_call("pm355_attn_kv4", c, _ATTN_KV4.pack(ty, n_head, q_at, ldq, out_at, ldo, scale, window, n_first, tiles.data_ptr(), of[0], tile_tokens, max_keys, T, w_at, w_n),
-                  torch._C._cuda_getCurrentRawStream(device))
+        try:
+            args = _ATTN_KV4.pack(ty, n_head, q_at, ldq, out_at, ldo, scale, window, n_first, tiles.data_ptr(), of[0], tile_tokens, max_keys, T, w_at, w_n)
+        except (struct.error, OverflowError) as e:
+            raise L.PM355Error("attn_kv4: %s" % e) from None
+        _kv4_call("pm355_attn_kv4", c, args, torch._C._cuda_getCurrentRawStream(device))
     return out
 
 

@@ -500,6 +500,18 @@ def test_refusals():
     assert ops.kv4_append(proj[:0], pages, table, pos[:0], pos[:0], H, G, d).shape == (0, H * d) and ops.attn_kv4(**{**good, "tiles": tiles[:0]}).shape == (3, H * d)
 
 
+@pytest.mark.parametrize("bad", [dict(window=1 << 32), dict(n_first=-1 << 40), dict(max_keys=1 << 31), dict(tile_tokens=1 << 31), dict(scale=1e39), dict(scale="1")])
+def test_numbers_that_do_not_fit(bad):
+    H, G, d = 4, 2, 64
+    z = lambda *n, t=torch.float32: torch.zeros(*n, dtype=t, device="cuda")  # noqa: E731
+    pages, table, tiles = z(2, ops.kv4_page_bytes(G, d), t=torch.uint8), z(1, 2, t=torch.int32), z(1, 4, t=torch.int32)
+    with pytest.raises(L.PM355Error):
+        ops.attn_kv4(**{**dict(q=z(3, H * d), pages=pages, table=table, tiles=tiles, tile_tokens=1, max_keys=4, n_head=H, n_head_kv=G, head_dim=d, scale=1.0), **bad})
+    if "scale" in bad:
+        with pytest.raises(L.PM355Error):
+            ops.kv4_append(z(3, (H + 2 * G) * d), pages, table, z(3, t=torch.int32), z(3, t=torch.int32), H, G, d, mscale=bad["scale"])
+
+
 # ---- together ---------------------------------------------------------------------------------------------------------------
 class Serving:
     """a model's cache as a program keeps it: pool, tables, pages of all layers"""

@@ -260,7 +260,7 @@ def test_nothing_to_do():
 @pytest.mark.parametrize("bad,code", [
     (dict(pairs=[(0, 4)]), RANGE), (dict(pairs=[(-1, 0)]), RANGE), (dict(pairs=[(0, 1), (2, 1)]), RANGE), (dict(pairs=[(0, 1), (1, 2)]), RANGE), (dict(pairs=[(2, 2)]), RANGE),
     (dict(page_bytes=24), ALIGN), (dict(page_bytes=0), SHAPE), (dict(layer_bytes=32 * 3), SHAPE), (dict(layer_bytes=32 * 4 + 8), ALIGN), (dict(pages=4104), ALIGN), (dict(pages=None), SHAPE),
-    (dict(n_layers=0), SHAPE), (dict(n_pages=0), SHAPE), (dict(n_pairs=-1), SHAPE)])
+    (dict(n_layers=0), SHAPE), (dict(n_pages=0), SHAPE), (dict(n_pairs=-1), SHAPE), (dict(n_pairs=5), SHAPE), (dict(n_pairs=1 << 30), SHAPE), (dict(n_pages=1 << 30), SHAPE)])
 def test_pages_copy_refused(bad, code):
     a = dict(pages=4096, page_bytes=32, layer_bytes=128, n_layers=2, n_pages=4, pairs=[(0, 1)])
     a.update(bad)
