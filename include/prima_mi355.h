@@ -470,7 +470,7 @@ typedef struct {
 PM355_API size_t pm355_kv4_page_bytes(int n_head_kv, int head_dim);      /* 0: sizes that are not supported */
 /* Norm, rotation and cache store of new tokens in one launch (llm_build_norm on heads + ggml_rope_ext + llm_build_kv_store): per head y = x / sqrt(mean(x^2) + eps) * norm (with
  * `norm`; norm_q / norm_k f32 [head_dim] or NULL: no weight), then the first n_rot dimensions turn by pos * d_turns[i] turns, pairs (2 i, 2 i + 1) or, with rope_neox, (i, i + n_rot / 2),
- * times mscale. Queries go to q (type, rounded once), keys - formed in 64 bits, so that their codes depend on no order of sums - and values into the pages. A row with d_pos < 0, d_seq
+ * times mscale (finite, like eps). Queries go to q (type, rounded once), keys - formed in 64 bits, so that their codes depend on no order of sums - and values into the pages. A row with d_pos < 0, d_seq
  * outside [0, n_seq), or without a page at its position stores nothing in the cache (its query is written; position 0 is taken where d_pos < 0). Rows of one call have different (sequence, position). q may be the
  * front of proj's own rows. */
 typedef struct {
@@ -487,7 +487,7 @@ PM355_API int pm355_kv4_load(const pm355_kv4_cache * c, const int32_t * d_pos, c
 /* Host: turns per position of each pair, freq_base^(-2 i / n_dims) / (2 pi), scaled like rope_yarn (ggml.c:14094-14131) and divided by freq_factors[i] (host, or NULL); *mscale likewise. In 64
  * bits, so that a position of 10^6 still has its angle to 10^-9. */
 PM355_API int pm355_rope_turns(const pm355_rope_params * rp, const float * freq_factors, double * turns, float * mscale);
-/* Attention over the pages: a query at position i sees the cached keys j <= i, with window > 0 those with i - j < window or j < n_first, on pages that are held; score = scale (q . k), softmax,
+/* Attention over the pages: a query at position i sees the cached keys j <= i, with window > 0 those with i - j < window or j < n_first, on pages that are held; score = scale (q . k) with a finite scale, softmax,
  * weighted values; 0 for a query that sees nothing (position < 0 among them). Queries come in tiles of consecutive tokens of one sequence, device int32 {row, tokens, position of the first,
  * sequence} each, of at most tile_tokens tokens. n_head / n_head_kv * tile_tokens <= 16, or tile_tokens == 1: decoded and drafted tokens, keys split over workgroups by max_keys (the
  * most keys that a tile sees; only the speed depends on it); up to 128: prompts. Keys and values are the cache's f16 values; queries and probabilities are f16 with type BF16 (queries

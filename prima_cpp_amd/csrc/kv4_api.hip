@@ -36,6 +36,7 @@ int pm355_kv4_append(const pm355_kv4_cache * c, const pm355_kv4_append_args * p,
         p->ldq < (int64_t) p->n_head * d || (int64_t) p->n_head * d > 0x0fffffff)
         return fail(PM355_E_SHAPE, "kv4_append: shape");
     if (p->d_turns && (p->n_rot < 8 || p->n_rot % 8 || p->n_rot > d)) return fail(PM355_E_SHAPE, "kv4_append: n_rot");
+    if (!isfinite(p->mscale) || !isfinite(p->eps)) return fail(PM355_E_RANGE, "kv4_append: mscale, eps");
     if (p->ld_proj % 4 || p->ldq % 4 || !aligned(p->proj, 16) || !aligned(p->q, 16)) return fail(PM355_E_ALIGN, "kv4_append: rows");
     (void) hipGetLastError();
     return done(pm_launch_kv4_append(cache_of(c), {p->type, p->n_head, p->n_tokens, p->proj, p->ld_proj, p->q, p->ldq, p->norm, p->norm_q, p->norm_k, p->eps, p->d_turns, p->n_rot, p->rope_neox, p->mscale,
@@ -77,6 +78,7 @@ int pm355_attn_kv4(const pm355_kv4_cache * c, const pm355_attn_kv4_args * p, pm3
         p->window < 0 || p->n_first < 0 || p->max_keys < 0)
         return fail(PM355_E_SHAPE, "attn_kv4: shape");
     if (p->tile_tokens < 1 || (p->tile_tokens > 1 && (int64_t) p->n_head / c->n_head_kv * p->tile_tokens > 128)) return fail(PM355_E_SHAPE, "attn_kv4: tile_tokens");
+    if (!isfinite(p->scale)) return fail(PM355_E_RANGE, "attn_kv4: scale");
     if ((int64_t) p->n_tiles * p->tile_tokens > 0x7fffffff) return fail(PM355_E_SHAPE, "attn_kv4: n_tiles");
     if (p->ldq % 8 || p->ldo % 8 || !aligned(p->q, 16) || !aligned(p->out, 16) || !aligned(p->d_tiles, 16) || !aligned(p->work, 16)) return fail(PM355_E_ALIGN, "attn_kv4: rows");
     (void) hipGetLastError();

@@ -239,7 +239,7 @@ def test_caches_refused(bad, code):
 @pytest.mark.parametrize("bad,code", [
     (dict(type=L.F16), UNSUPPORTED), (dict(type=99), UNSUPPORTED), (dict(n_tokens=-1), SHAPE), (dict(n_head=3), SHAPE), (dict(n_head=0), SHAPE), (dict(proj=None), SHAPE), (dict(q=None), SHAPE),
     (dict(d_pos=None), SHAPE), (dict(d_seq=None), SHAPE), (dict(ld_proj=508), SHAPE), (dict(ldq=252), SHAPE), (dict(ld_proj=514), ALIGN), (dict(ldq=258), ALIGN), (dict(proj=4104), ALIGN),
-    (dict(q=4100), ALIGN), (dict(d_turns=4096, n_rot=0), SHAPE), (dict(d_turns=4096, n_rot=12), SHAPE), (dict(d_turns=4096, n_rot=72), SHAPE)])
+    (dict(q=4100), ALIGN), (dict(d_turns=4096, n_rot=0), SHAPE), (dict(d_turns=4096, n_rot=12), SHAPE), (dict(d_turns=4096, n_rot=72), SHAPE), (dict(mscale=float("inf")), RANGE), (dict(eps=float("nan")), RANGE)])
 def test_append_refused(bad, code):
     assert append(**bad) == code
 
@@ -248,7 +248,7 @@ def test_append_refused(bad, code):
     (dict(type=L.F16), UNSUPPORTED), (dict(n_tiles=-1), SHAPE), (dict(n_tokens=0), SHAPE), (dict(n_head=5), SHAPE), (dict(q=None), SHAPE), (dict(out=None), SHAPE), (dict(d_tiles=None), SHAPE),
     (dict(ldq=248), SHAPE), (dict(ldo=248), SHAPE), (dict(window=-1), SHAPE), (dict(n_first=-1), SHAPE), (dict(max_keys=-1), SHAPE), (dict(tile_tokens=0), SHAPE), (dict(tile_tokens=65), SHAPE),
     (dict(ldq=260), ALIGN), (dict(ldo=260), ALIGN), (dict(q=4104), ALIGN), (dict(out=4104), ALIGN), (dict(d_tiles=4100), ALIGN), (dict(work=4100, work_floats=9), ALIGN),
-    (dict(n_tiles=2 ** 30, tile_tokens=4), SHAPE)])
+    (dict(n_tiles=2 ** 30, tile_tokens=4), SHAPE), (dict(scale=float("nan")), RANGE), (dict(scale=float("-inf")), RANGE)])
 def test_attend_refused(bad, code):
     assert attend(**bad) == code
 
