@@ -673,12 +673,18 @@ template <typename T, int D, int COLS> __global__ __launch_bounds__(256) void jo
 
 // FEW_WANT: one workgroup of 8 waves per CU is enough to fill the memory's queues, and every split costs its join. 32 tokens of 8 KV heads behind 8190 keys: 256 workgroups 67 us, 512 73, 1024 (of
 // 4 waves) 80; one token behind 262100: 72, 72, 82. FEW_COLS: up to there rows of keys are read again per 32 columns; 8 x 16 tokens x 4 heads behind 4000 34 us, as one tile of 128 columns 38.
-// TILES_WANT: 64 tokens behind 30000 58 us, with 256 61; 512 behind 8000 108 and 119. LEAST: pages that a split is worth (204 keys in 2 splits 10.5 us, in one 7.5).
-constexpr int FEW_WANT = 256, FEW_LEAST = 4, FEW_MOST = 128, FEW_COLS = 64, TILES_WANT = 512, TILES_LEAST = 8, TILES_MOST = 32;
+// FEW_PAGES: wider tiles go that way too where their workgroups are one round and all of them together read no more pages than this. 64, 128, 256 tokens of 32 + 8 heads of 128: behind 500 16, 19,
+// 16 us, as tiles 23, 24, 28; behind 2000 21, 26, 30 and 26, 29, 34; behind 4000 (1040, 2080, 4224 pages) 25, 34, 46 and 27, 31, 43. 512 tokens (512 workgroups) 26 us, as tiles 21.
+// FEW_JOIN: a join costs as much as FEW_JOIN / d + 2 pages of a workgroup, which the splits have to save. One token of 8 KV heads of 128 behind 500, 700, 1000, 1500: 9.0, 10.4, 11.7, 14.7 us in one,
+// 11.4 .. 11.5 split; of 64: 7.4, 8.3, 9.2, 11.2 and 10.5 .. 10.8; of 256: 12.7, 15.1, 17.1, 21.4 and 13.7 .. 14.0.
+// TILES_WANT: two workgroups per CU (one from heads of 192 on) share its matrix cores: 1.6 times the time of one, not 2. 512 tokens of 32 + 8 heads of 128 behind 12000 147 us, with 256 167. Partial sums
+// are written and read, 2 * 128 (d + 2) floats per split, so splits have to save 3 pages and one more per 54 of them: 1000 tokens behind 300 42 us, in 2 splits 55; behind 12000 293 and 272; 320
+// behind 900 34 in one, 28 in 6; 512 of 16 + 4 heads of 256 behind 4000 97 in 4, 81 in 2. LEAST: a step for every wave; a page's work for a join.
+constexpr int FEW_WANT = 256, FEW_LEAST = 4, FEW_MOST = 128, FEW_COLS = 64, FEW_PAGES = 1536, FEW_JOIN = 1100, TILES_WANT = 512, TILES_LEAST = 4, TILES_MOST = 32;
 // workgroups over which the keys of a slot are split: as many as fill the chip, none with less than `least` pages, and what the scratch holds
 int splits_of(const pm_kv4_attn & a, int64_t slots, int64_t busy, int want, int least, int most, int64_t floats) {
     const int64_t pages = ((int64_t) a.max_keys + PM_PAGE - 1) / PM_PAGE, room = a.work ? (int64_t) a.work_floats / (slots * floats) : 1;
-    int64_t n = (want + busy - 1) / busy;
+    int64_t n = want / busy;                               // (rounded up, the last ones are a second round: 6 tokens of 8 KV heads behind 8000 27 us instead of 22)
     n = n < pages / least ? n : pages / least;
     n = n < room ? n : room;
     n = n < most ? n : most;
@@ -695,13 +701,17 @@ template <typename T, int NB> int launch(const pm_kv4_cache & c, pm_kv4_attn a, 
     constexpr bool WIDE = sizeof(T) == 4;
     const int R = a.H / c.G;
     if (a.window > 0) { const int64_t most = (int64_t) a.window + a.tile_tokens + 128 + a.first; if (most < a.max_keys) a.max_keys = (int) most; }
+    const int64_t pages = ((int64_t) a.max_keys + PM_PAGE - 1) / PM_PAGE;
     // columns of a tile on the average: tile_tokens only bounds them
     const int64_t cols = (int64_t) R * (a.n_tokens / a.n_tiles < a.tile_tokens ? (a.n_tokens + a.n_tiles - 1) / a.n_tiles : a.tile_tokens);
     auto few = [&](auto kern, auto ctc) -> int {
         constexpr int ct = decltype(ctc)::value;
-        const int passes = (R * a.tile_tokens + 16 * ct - 1) / (16 * ct), launched = ct > 1 ? (int) ((cols + 16 * ct - 1) / (16 * ct)) : passes;
+        // (all passes side by side where that is one round and most of them have work: 40 tokens in tiles of 32 behind 100 11 us, with as many workgroups as the average wants 18)
+        const int passes = (R * a.tile_tokens + 16 * ct - 1) / (16 * ct), average = (int) ((cols + 16 * ct - 1) / (16 * ct));
+        const int launched = ct > 1 && (average * 2 <= passes || (int64_t) a.n_tiles * c.G * passes > FEW_WANT) ? average : passes;
         const int64_t slots = (int64_t) a.n_tiles * c.G * passes, busy = (int64_t) a.n_tiles * c.G * launched;
-        const int splits = splits_of(a, slots, busy, FEW_WANT, FEW_LEAST, FEW_MOST, 16 * ct * (D + 2));
+        int splits = splits_of(a, slots, busy, FEW_WANT, FEW_LEAST, FEW_MOST, 16 * ct * (D + 2));
+        if ((pages - (pages + splits - 1) / splits - 2) * D < FEW_JOIN) splits = 1;
         if (busy * splits >= 1 << 23 || slots >= 1 << 20) return PM355_E_SHAPE;      // (a launch has fewer than 2^32 threads, that of the joins up to 16 workgroups of 256 per slot)
         const size_t ring = (size_t) FW * STAGES * pm_step<NB>::BYTES, acc = (size_t) FW * 16 * (D + 4) * 4, lds = ring > acc ? ring : acc;
         pm_allow_big_lds((const void *) kern, lds);
@@ -709,12 +719,15 @@ template <typename T, int NB> int launch(const pm_kv4_cache & c, pm_kv4_attn a, 
         if (splits > 1) join<T, D, 16 * ct>(c, a, slots, passes, splits, st);
         return 0;
     };
-    if (a.tile_tokens == 1 || cols <= FEW_COLS) {
-        if constexpr (NB <= (WIDE ? 3 : 4)) if (cols > 16) return few(few_kernel<T, NB, WIDE, 2>, std::integral_constant<int, 2>());
+    constexpr int CT = NB <= (WIDE ? 3 : 4) ? 2 : 1;
+    const int64_t tiles = (int64_t) a.n_tiles * c.G;
+    if (a.tile_tokens == 1 || cols <= FEW_COLS || (tiles * ((cols + 16 * CT - 1) / (16 * CT)) <= FEW_WANT && tiles * pages <= FEW_PAGES)) {
+        if constexpr (CT == 2) if (cols > 16) return few(few_kernel<T, NB, WIDE, 2>, std::integral_constant<int, 2>());
         return few(few_kernel<T, NB, WIDE, 1>, std::integral_constant<int, 1>());
     }
     const int64_t slots = (int64_t) a.n_tiles * c.G;
-    const int splits = splits_of(a, slots, slots, TILES_WANT, TILES_LEAST, TILES_MOST, TC * (D + 2));
+    int splits = splits_of(a, slots, slots, NB <= 4 ? TILES_WANT : TILES_WANT / 2, TILES_LEAST, TILES_MOST, TC * (D + 2));
+    if (pages - (slots * splits > TILES_WANT / 2 ? 1.6 : 1.0) * (double) ((pages + splits - 1) / splits) < 3.0 + (double) (slots * splits) / 54.0) splits = 1;
     const size_t lds = 2 * ((size_t) PM_PAGE * (D * 2 + 16) + D * (PM_PAGE * 2 + 16));
     if (slots * splits >= 1 << 24 || (splits > 1 && slots >= 1 << 17)) return PM355_E_SHAPE;
     static_assert(2 * (PM_PAGE * (D * 2 + 16) + D * (PM_PAGE * 2 + 16)) >= TC * (D + 4) * 4, "the partial sums go through the pages' LDS");
