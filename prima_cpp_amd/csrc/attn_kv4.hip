@@ -5,8 +5,8 @@
 // ordered so that a mask gives a pair that an operand wants). Queries are brought to [1, 2) by a power of two per row, exact for bf16; WIDE (32-bit rows) holds queries and probabilities as
 // pairs of f16 and makes two products of each. Probabilities are held times 2^8, so that f16 has its steps of 2^-11 down to p = 2^-22.
 // S^T = K Q^T is computed with the key rows permuted so that a lane's score registers are its P operand of O^T = V^T P^T.
-//   few    16 or 32 columns (tokens x query heads of a KV head) per workgroup, 32 keys per wave and step, keys split over waves and workgroups: bound by memory. 48 tokens of 64 heads behind
-//          3300 .. 8203 keys 74 us (329 MB, 4.4 TB/s), one of 32 heads behind 131100 36 us (151 MB), 16 x 4 of 28 heads in a window of 4096 24 us; a large copy reaches 4.9 TB/s here
+//   few    16 or 32 columns (tokens x query heads of a KV head) per workgroup, 32 keys per wave and step, keys split over waves and workgroups: bound by memory, short prompt portions by the way
+//          through one step. 48 tokens of 64 heads behind 3300 .. 8203 keys 74 us (329 MB, 4.4 TB/s), one of 32 heads behind 131100 37 us (151 MB), 16 x 4 of 28 heads in a window of 4096 24 us; a large copy reaches 4.9 TB/s here
 //   tiles  128 columns per workgroup, a page at a time through LDS, where it is made f16 once for all four waves: bound by the matrix cores, which run at 1.1 .. 1.3 PFLOP/s under load.
 //          4096 tokens of 32 heads behind 2011: 316 us, 860 TFLOP/s (a large f16 product of the library 1110)
 //   join   the partial sums of split keys
