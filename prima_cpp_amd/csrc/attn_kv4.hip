@@ -90,12 +90,14 @@ __device__ __forceinline__ void split_f16(const float * x, f16x8 & hi, f16x8 & l
 #pragma unroll
     for (int j = 0; j < 8; ++j) { hi[j] = (_Float16) x[j]; lo[j] = (_Float16) (x[j] - (float) hi[j]); }
 }
-// 2^-e with the sign of scale for a row whose largest magnitude is in [2^e, 2^(e + 1)); cf = |scale| log2(e) 2^e, up to 2^100: scores (below 2^25) differ by 2^-48 at the least
+// 2^-e with the sign of scale for a row whose largest magnitude is in [2^e, 2^(e + 1)); cf = |scale| log2(e) 2^e, up to 2^100: scores (below 2^25) differ by 2^-48 at the least.
+// NaN for a row with an infinity: whatever keys it meets its softmax is NaN, but scores of nothing but -inf would pass for keys that are hidden
 __device__ __forceinline__ float row_factor(float most, float scale, float & cf) {
     int e = (int) (__builtin_bit_cast(uint32_t, most) >> 23 & 255) - 127;
-    e = e < -100 ? -100 : e > 127 ? 0 : e;                 // (a row of zeros; rows that are not finite stay so)
+    const bool finite = e < 128;
+    e = e < -100 ? -100 : finite ? e : 0;                  // (a row of zeros)
     cf = fminf(fmaxf(fabsf(scale) * LOG2E * ldexpf(1.0f, e), 1e-30f), 0x1p100f);
-    return copysignf(ldexpf(1.0f, -e), scale);
+    return finite ? copysignf(ldexpf(1.0f, -e), scale) : NAN;
 }
 
 // what the columns of a tile see together: pages [0, front) and from p0 on, `count` in all
