@@ -95,8 +95,8 @@ __device__ __forceinline__ void split_f16(const float * x, f16x8 & hi, f16x8 & l
 __device__ __forceinline__ float row_factor(float most, float scale, float & cf) {
     int e = (int) (__builtin_bit_cast(uint32_t, most) >> 23 & 255) - 127;
     const bool finite = e < 128;
-    e = e < -100 ? -100 : finite ? e : 0;                  // (a row of zeros)
-    cf = fminf(fmaxf(fabsf(scale) * LOG2E * ldexpf(1.0f, e), 1e-30f), 0x1p100f);
+    e = finite ? e : 0;                                    // (-127: zeros, and numbers below 2^-126)
+    cf = fminf(fmaxf(fabsf(scale) * ldexpf(1.0f, e) * LOG2E, 1e-30f), 0x1p100f);      // (in this order nothing on the way leaves 32 bits that the end does not)
     return finite ? copysignf(ldexpf(1.0f, -e), scale) : NAN;
 }
 

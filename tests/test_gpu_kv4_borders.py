@@ -50,3 +50,17 @@ def test_queries_that_are_not_finite_and_see_nothing(n, type):
     q = torch.full((2 * n, H * d), float("inf"), device="cuda", dtype=TYPES[type])
     tiles = dev(np.array([(0, n, -n, 0), (n, n, 3, 9)], np.int32))
     assert not ops.attn_kv4(q, dev(random_pages(2, G, d, r)), dev(np.array([[0, 1]], np.int32)), tiles, n, 128, H, G, d, 1.0).any()
+
+
+@pytest.mark.parametrize("type", ["bf16", "f32"])
+@pytest.mark.parametrize("gain,scale", [(1e-36, 1e35), (3e-33, 3e38), (5e37, 2e-39), (1e-20, 9e18), (1e-38, 3e38), (1e-39, 3e38)])
+@pytest.mark.parametrize("batch", list(BATCHES))
+def test_queries_and_scales_of_any_size(batch, gain, scale, type):
+    """the smallest and largest queries with the scale that makes ordinary scores of them: nothing of either is lost on the way"""
+    H, G, d = 16, 16, 128
+    entries, r = BATCHES[batch], np.random.default_rng(3)
+    table, n = tables([p + m for _, p, m in entries], r)
+    raw = random_pages(n, G, d, r)
+    q = torch.from_numpy((gain * r.normal(size=(rows(entries), H * d))).astype(np.float32)).to(TYPES[type]).cuda()
+    assert torch.isfinite(q).all()
+    A.compare(run(q, raw, table, entries, H, G, d, scale), *A.expected(q, raw, table, entries, H, G, d, scale))
