@@ -175,9 +175,20 @@ template <typename T, int NB> __global__ __launch_bounds__(256) void append_kern
             float ss = 0.0f;
 #pragma unroll
             for (int j = 0; j < 8; ++j) ss = fmaf(x[j], x[j], ss);
-            const float r = __builtin_amdgcn_rsqf(head_sum<LPH>(ss) * (1.0f / D) + a.eps);
+            const float mean = head_sum<LPH>(ss) * (1.0f / D) + a.eps, r = __builtin_amdgcn_rsqf(mean);      // (v_rsq_f32: 1 unit of 2^-23)
+            // squares that leave 32 bits - values beyond 10^19, or below 10^-15 without an eps that says more - are summed in 64, like those of keys
+            const bool odd = !(mean > 1e-30f && mean < 1e30f);
+            if (__any(live && odd)) {
+                double s2 = 0.0;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] *= r * w[j];
+                for (int j = 0; j < 8; ++j) s2 = fma((double) x[j], (double) x[j], s2);
+                const double r2 = 1.0 / sqrt(head_sum<LPH>(s2) / D + (double) a.eps);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[j] = odd ? (float) (x[j] * r2 * w[j]) : x[j] * (r * w[j]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[j] *= r * w[j];
+            }
         }
         if (rot) {
             if (a.neox)

@@ -64,3 +64,27 @@ def test_queries_and_scales_of_any_size(batch, gain, scale, type):
     q = torch.from_numpy((gain * r.normal(size=(rows(entries), H * d))).astype(np.float32)).to(TYPES[type]).cuda()
     assert torch.isfinite(q).all()
     A.compare(run(q, raw, table, entries, H, G, d, scale), *A.expected(q, raw, table, entries, H, G, d, scale))
+
+
+@pytest.mark.parametrize("type", ["bf16", "f32"])
+@pytest.mark.parametrize("d,H,G,T", [(64, 5, 1, 9), (96, 4, 2, 9), (128, 12, 3, 9), (256, 8, 2, 9), (128, 12, 3, 700)])
+@pytest.mark.parametrize("eps", [0.0, 1e-6])
+def test_norms_of_any_size(eps, d, H, G, T, type):
+    """queries and keys whose squares leave 32 bits at either end have norms like others; a row of zeros stays zeros where eps is not 0"""
+    r = np.random.default_rng(d + T)
+    sizes = np.array([1.0, 1e19, 3e25, 4e37, 1e-12, 1e-20, 1e-24, 1e-37, 0.0 if eps else 1e-30])[np.arange(T) % 9]
+    x = r.normal(size=(T, H + 2 * G, d)) * sizes[:, None, None]
+    x[T // 2, ::2] *= 1e-8                                   # heads of unlike sizes in one token
+    proj = torch.from_numpy(x.reshape(T, -1).astype(np.float32)).to(TYPES[type])
+    wq, wk = (torch.from_numpy(r.uniform(0.5, 1.5, d).astype(np.float32)) for _ in range(2))
+    pages = torch.zeros(T // 64 + 1, ops.kv4_page_bytes(G, d), dtype=torch.uint8, device="cuda")
+    args = (pages, torch.arange(T // 64 + 1, dtype=torch.int32, device="cuda")[None], torch.arange(T, dtype=torch.int32, device="cuda"), torch.zeros(T, dtype=torch.int32, device="cuda"))
+    q = ops.kv4_append(proj.cuda(), *args, H, G, d, norm=True, norm_q=wq.cuda(), norm_k=wk.cuda(), eps=eps).float().cpu().numpy().reshape(T, H, d)
+    k = ops.kv4_load(*args, G, d)[0].cpu().numpy()
+    x, half, eps = proj.float().numpy().reshape(T, -1, d), torch.finfo(TYPES[type]).eps / 2, float(np.float32(eps))
+    for t in range(T) if T < 10 else (0, 1, 2, 3, 6, 8, 66, T // 2, T - 1):
+        for h in range(H):
+            e = P.norm_rotate(x[t, h], wq.numpy(), True, eps, 0, None, 1.0, False)
+            assert (np.abs(q[t, h] - e) <= half * np.abs(e) + 2e-6 * np.abs(e).max()).all(), (t, h, q[t, h, :4], e[:4])
+        for g in range(G):
+            assert np.array_equal(k[t, g], P.values(*P.quantize(P.norm_rotate(x[t, H + g], wk.numpy(), True, eps, 0, None, 1.0, False).astype(np.float32)))), (t, g)
