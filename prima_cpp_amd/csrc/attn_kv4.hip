@@ -168,7 +168,7 @@ template <typename T, int NB, bool WIDE, int CT> __global__ __launch_bounds__(FW
     // (tiles may have more columns than they have on the average, for which the launch is made: with CT > 1 a workgroup takes the further ones too. Workgroups without work are no way
     // out: each waits for its LDS behind those that work)
     int pass = id / G % launched;
-    if (pass * COLS >= n * R) return;
+    if (n < 1 || pass * COLS >= n * R) return;             // (what a tile's count is times R may leave 32 bits where it is negative)
     do {
     const size_t slot = ((size_t) at * passes + pass) * G + g;
     const int col0 = pass * COLS, left = n * R - col0, cols = left < COLS ? left : COLS;
@@ -615,7 +615,7 @@ template <typename T, int D, int COLS> __global__ __launch_bounds__(256) void jo
     const int g = slot % G, pass = slot / G % passes;
     const int32_t * tile = uniform_const_ptr(a.tiles) + slot / G / passes * 4;
     const int row0 = tile[0], n = tile[1] < a.tile_tokens ? tile[1] : a.tile_tokens, room = COLS - first < each ? COLS - first : each, left = n * R - pass * COLS - first, cols = left < room ? left : room;
-    if (cols < 1) return;
+    if (n < 1 || cols < 1) return;
     const float * part = a.work + slot * splits * COLS * (D + 2) + first * D, * part_ml = a.work + slot * splits * COLS * (D + 2) + (size_t) splits * COLS * D + first * 2;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, items = cols * (D / 4), groups = items < 256 ? 256 / items : 1;
     // the first splits of this thread's column are on their way while the factors are formed

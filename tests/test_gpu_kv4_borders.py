@@ -88,3 +88,19 @@ def test_norms_of_any_size(eps, d, H, G, T, type):
             assert (np.abs(q[t, h] - e) <= half * np.abs(e) + 2e-6 * np.abs(e).max()).all(), (t, h, q[t, h, :4], e[:4])
         for g in range(G):
             assert np.array_equal(k[t, g], P.values(*P.quantize(P.norm_rotate(x[t, H + g], wk.numpy(), True, eps, 0, None, 1.0, False).astype(np.float32)))), (t, g)
+
+
+@pytest.mark.parametrize("R", [1, 3, 5])
+def test_tiles_without_tokens(R):
+    """counts of 0, -1 and of numbers whose products with the heads of a KV head leave 32 bits: nothing is written, and the scratch behind the slots stays as it is"""
+    G, d, r = 2, 64, np.random.default_rng(R)
+    H, q = G * R, torch.randn(3, G * R * 64, device="cuda")
+    table, n = tables([9000, 300], r)
+    raw = random_pages(n, G, d, r)
+    counts = [0, -1, -2 ** 31, -2 ** 30, -715827883, -858993460, -429496730, -1431655765]
+    for tile in (1, 16 // R, 128 // R):
+        tiles = dev(np.array([(1, c, 5, 1) for c in counts] + [(0, 1, 8999, 0)], np.int32))
+        out, work = torch.full((3, H * d), 5.0, device="cuda"), torch.full((1 << 22,), 7.0, device="cuda")
+        ops.attn_kv4(q, dev(raw), dev(table), tiles, tile, 9000, H, G, d, 0.125, out=out, work=work)
+        A.compare(out[:1], *A.expected(q[:1], raw, table, [(0, 8999, 1)], H, G, d, 0.125))
+        assert (out[1:] == 5.0).all() and (work[1 << 21:] == 7.0).all()
