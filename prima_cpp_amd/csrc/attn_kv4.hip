@@ -606,10 +606,11 @@ template <typename T, int NB, bool WIDE> __global__ __launch_bounds__(256, NB <=
 
 // ---- joining split keys: partial sums per slot [splits][COLS][D], then [splits][COLS][maximum, sum]. A launch of its own: the workgroup of a slot that ends last could do it too, but it
 // reads 2 MB (128 columns, 32 splits) alone, and waits for three trips to memory that other XCDs have written to; 64 tokens behind 30000 took 118 us that way ------------------------------
+__host__ __device__ constexpr size_t join_factors(int splits, int each) { return ((size_t) splits * each * 8 + 15) & ~(size_t) 15; }      // bytes
 template <typename T, int D, int COLS> __global__ __launch_bounds__(256) void join_kernel(pm_kv4_cache c, pm_kv4_attn a, int passes, int splits, int each) {
-    extern __shared__ __attribute__((aligned(16))) char lds_j[];          // [splits][each][factor, sum], then the sums of groups of splits
+    extern __shared__ __attribute__((aligned(16))) char lds_j[];          // [splits][each][factor, sum], then the sums of groups of splits, at a multiple of 16 bytes
     __shared__ float inv[COLS];
-    float * ml = (float *) lds_j, * sums = ml + splits * each * 2;
+    float * ml = (float *) lds_j, * sums = (float *) (lds_j + join_factors(splits, each));
     const int blocks = (COLS + each - 1) / each, first = blockIdx.x % blocks * each, G = c.G, R = a.H / G;
     const size_t slot = blockIdx.x / blocks;
     const int g = slot % G, pass = slot / G % passes;
@@ -696,7 +697,7 @@ int splits_of(const pm_kv4_attn & a, int64_t slots, int64_t busy, int want, int 
 // columns per workgroup: the joined values of a thread come from about 16 splits
 template <typename T, int D, int COLS> void join(const pm_kv4_cache & c, const pm_kv4_attn & a, int64_t slots, int passes, int splits, hipStream_t st) {
     const int most = 1024 / D, want = 16384 / (D * splits), each = want < 1 ? 1 : want < most ? want : most;
-    hipLaunchKernelGGL((join_kernel<T, D, COLS>), dim3((unsigned) (slots * ((COLS + each - 1) / each))), dim3(256), (size_t) splits * each * 8 + 4096, st, c, a, passes, splits, each);
+    hipLaunchKernelGGL((join_kernel<T, D, COLS>), dim3((unsigned) (slots * ((COLS + each - 1) / each))), dim3(256), join_factors(splits, each) + 4096, st, c, a, passes, splits, each);
 }
 template <typename T, int NB> int launch(const pm_kv4_cache & c, pm_kv4_attn a, hipStream_t st) {
     constexpr int D = NB * 32;
