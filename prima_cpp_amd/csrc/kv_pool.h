@@ -14,9 +14,10 @@ struct pm355_page_pool {
     std::vector<int> free_list;
     std::vector<int> users;                                // tables that hold the page, 0: free
     std::vector<Seq> seqs;
+    const bool keeps_changes;                              // for an owner that takes them step by step (the C entries do not: there they would only grow)
     std::vector<std::pair<int, int>> changes;              // (seq * max_seq_pages + index, page) since the owner last took them
 
-    pm355_page_pool(int pages, int n_seqs, int max_pages) : n_pages(pages), max_seq_pages(max_pages), users((size_t) pages), seqs((size_t) n_seqs) {
+    pm355_page_pool(int pages, int n_seqs, int max_pages, bool keep) : n_pages(pages), max_seq_pages(max_pages), users((size_t) pages), seqs((size_t) n_seqs), keeps_changes(keep) {
         for (int i = pages - 1; i >= 0; --i) free_list.push_back(i);
     }
     bool valid(int s) const { return s >= 0 && s < (int) seqs.size() && seqs[s].open; }
@@ -24,7 +25,8 @@ struct pm355_page_pool {
         for (size_t s = 0; s < seqs.size(); ++s) if (!seqs[s].open) { seqs[s] = Seq(); seqs[s].open = true; return (int) s; }
         return PM355_E_NOMEM;
     }
-    void room(size_t n) { if (changes.capacity() < changes.size() + n) changes.reserve(std::max(2 * changes.capacity(), changes.size() + n)); }
+    void room(size_t n) { if (keeps_changes && changes.capacity() < changes.size() + n) changes.reserve(std::max(2 * changes.capacity(), changes.size() + n)); }
+    void changed(int s, int i) { if (keeps_changes) changes.push_back({s * max_seq_pages + i, seqs[s].page[i]}); }      // (behind room())
     void release(int page) { if (page >= 0 && --users[page] == 0) free_list.push_back(page); }
     int close(int s) {
         if (!valid(s)) return PM355_E_RANGE;
@@ -45,7 +47,7 @@ struct pm355_page_pool {
             seqs[s].page.push_back(free_list.back());
             free_list.pop_back();
             users[seqs[s].page.back()] = 1;
-            changes.push_back({s * max_seq_pages + seqs[s].hi++, seqs[s].page.back()});
+            changed(s, seqs[s].hi++);
         }
         return 0;
     }
@@ -76,7 +78,7 @@ struct pm355_page_pool {
         q.hi = hi;
         q.lo = std::min(seqs[s].lo, hi);
         q.page.swap(held);
-        for (int i = q.lo; i < q.hi; ++i) if (q.page[i] >= 0) { ++users[q.page[i]]; changes.push_back({t * max_seq_pages + i, q.page[i]}); }
+        for (int i = q.lo; i < q.hi; ++i) if (q.page[i] >= 0) { ++users[q.page[i]]; changed(t, i); }
         return t;
     }
     // pages of s from the one of position `from` on that others hold too become its own; pairs (from, to) of what has to be copied
@@ -94,7 +96,7 @@ struct pm355_page_pool {
             free_list.pop_back();
             *pairs++ = q.page[i]; *pairs++ = to;
             --users[q.page[i]]; users[to] = 1; q.page[i] = to;
-            changes.push_back({s * max_seq_pages + i, to});
+            changed(s, i);
         }
         return n;
     }
@@ -117,7 +119,7 @@ struct pm355_page_pool {
         for (size_t s = 0; s < seqs.size(); ++s)
             for (int i = seqs[s].lo; i < seqs[s].hi; ++i) {
                 int & p = seqs[s].page[i];
-                if (p >= 0 && to[p] >= 0) { p = to[p]; changes.push_back({(int) s * max_seq_pages + i, p}); }
+                if (p >= 0 && to[p] >= 0) { p = to[p]; changed((int) s, i); }
             }
         free_list.clear();
         for (int i = n_pages - 1; i >= used; --i) free_list.push_back(i);

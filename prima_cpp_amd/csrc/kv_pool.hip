@@ -7,7 +7,7 @@ template <class F> static int guarded(F && f) { try { return f(); } catch (...) 
 
 extern "C" {
 pm355_page_pool * pm355_page_pool_new(int n_pages, int n_seqs, int max_seq_pages) {
-    try { return n_pages > 0 && n_seqs > 0 && max_seq_pages > 0 ? new pm355_page_pool(n_pages, n_seqs, max_seq_pages) : nullptr; } catch (...) { return nullptr; }
+    try { return n_pages > 0 && n_seqs > 0 && max_seq_pages > 0 ? new pm355_page_pool(n_pages, n_seqs, max_seq_pages, false) : nullptr; } catch (...) { return nullptr; }
 }
 void pm355_page_pool_free(pm355_page_pool * p) { delete p; }
 int pm355_page_pool_open(pm355_page_pool * p) { return p->open(); }

@@ -489,7 +489,7 @@ int pm_stack::finalize_pool(int max_tokens_, int n_seq, int64_t pool_tokens) {
         if (hipHostMalloc((void **) &h_meta[i], meta_ints * 4, hipHostMallocDefault) != hipSuccess || hipEventCreateWithFlags(&h_free[i], hipEventDisableTiming) != hipSuccess)
             return fail(PM355_E_NOMEM, "finalize: pinned step tables");
     if (!cap_stream && hipStreamCreateWithFlags(&cap_stream, hipStreamNonBlocking) != hipSuccess) return fail(PM355_E_HIP, "finalize: capture stream");
-    pool = new pm355_page_pool(pages, n_seq, seq_pages);
+    pool = new pm355_page_pool(pages, n_seq, seq_pages, true);
     len.assign(n_seq, 0);
     max_tokens = max_tokens_;
     return hipDeviceSynchronize() == hipSuccess ? 0 : fail(PM355_E_HIP, "finalize");
