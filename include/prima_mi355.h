@@ -503,6 +503,9 @@ typedef struct {
 } pm355_attn_kv4_args;
 PM355_API size_t pm355_attn_kv4_work_floats(int n_head, int n_head_kv, int head_dim);
 PM355_API int pm355_attn_kv4(const pm355_kv4_cache * c, const pm355_attn_kv4_args * a, pm355_stream_t stream);
+/* What that call launches - host arithmetic only, no device needed, with the same refusals: out4 = {columns (tokens x query heads of a KV head) per workgroup: 16 or 32 (the kernel for few) or 128
+ * (the one for prompts), workgroups side by side over the columns of a tile, workgroups that share the keys, workgroups in all (fewer than 2^23, for prompts than 2^24: more are refused)}. */
+PM355_API int pm355_attn_kv4_plan(const pm355_kv4_cache * c, const pm355_attn_kv4_args * a, int32_t * out4);
 /* Pages of a pool copied in every layer: for each (from, to) of n_pairs host pairs, pages[layer][to] = pages[layer][from], page_bytes (a multiple of 16) each, layers layer_bytes apart. Every
  * `to` stands once and is no `from` (llama_kv_cache_seq_cp and llama_kv_cache_defrag move cells, src/llama.cpp:4183, :4334). The pairs travel with the launch. */
 PM355_API int pm355_pages_copy(void * pages, size_t page_bytes, size_t layer_bytes, int n_layers, int n_pages, const int32_t * pairs, int n_pairs, pm355_stream_t stream);

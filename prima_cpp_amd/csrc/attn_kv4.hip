@@ -13,7 +13,6 @@
 #include "pm355_kv4.h"
 #include "pm355_kernels.h"
 #include "../../include/prima_mi355.h"
-#include <type_traits>
 
 namespace {
 
@@ -685,58 +684,72 @@ template <typename T, int D, int COLS> __global__ __launch_bounds__(256) void jo
 // behind 900 34 in one, 28 in 6; 512 of 16 + 4 heads of 256 behind 4000 97 in 4, 81 in 2. LEAST: a step for every wave; a page's work for a join.
 constexpr int FEW_WANT = 256, FEW_LEAST = 4, FEW_MOST = 128, FEW_COLS = 64, FEW_PAGES = 1536, FEW_JOIN = 1100, TILES_WANT = 512, TILES_LEAST = 4, TILES_MOST = 32;
 // workgroups over which the keys of a slot are split: as many as fill the chip, none with less than `least` pages, and what the scratch holds
-int splits_of(const pm_kv4_attn & a, int64_t slots, int64_t busy, int want, int least, int most, int64_t floats) {
-    const int64_t pages = ((int64_t) a.max_keys + PM_PAGE - 1) / PM_PAGE, room = a.work ? (int64_t) a.work_floats / (slots * floats) : 1;
+int splits_of(const pm_kv4_attn & a, int64_t pages, int64_t slots, int64_t busy, int want, int least, int most, int64_t floats) {
+    const int64_t room = a.work ? (int64_t) a.work_floats / (slots * floats) : 1;
     int64_t n = want / busy;                               // (rounded up, the last ones are a second round: 6 tokens of 8 KV heads behind 8000 27 us instead of 22)
     n = n < pages / least ? n : pages / least;
     n = n < room ? n : room;
     n = n < most ? n : most;
     return n < 1 ? 1 : (int) n;
 }
+constexpr int columns_of(int nb, bool wide) { return nb <= (wide ? 3 : 4) ? 2 : 1; }       // tiles of 16 columns that a workgroup of few_kernel has registers for
+pm_kv4_plan plan_of(int nb, bool wide, const pm_kv4_cache & c, const pm_kv4_attn & a) {
+    const int R = a.H / c.G, D = nb * 32, CT = columns_of(nb, wide);
+    const int64_t seen = (int64_t) a.window + a.tile_tokens + 128 + a.first, keys = a.window > 0 && seen < a.max_keys ? seen : a.max_keys, pages = (keys + PM_PAGE - 1) / PM_PAGE;
+    // columns of a tile on the average: tile_tokens only bounds them
+    const int64_t cols = (int64_t) R * (a.n_tokens / a.n_tiles < a.tile_tokens ? (a.n_tokens + a.n_tiles - 1) / a.n_tiles : a.tile_tokens), tiles = (int64_t) a.n_tiles * c.G;
+    pm_kv4_plan p{};
+    if (a.tile_tokens == 1 || cols <= FEW_COLS || (tiles * ((cols + 16 * CT - 1) / (16 * CT)) <= FEW_WANT && tiles * pages <= FEW_PAGES)) {
+        const int ct = cols > 16 ? CT : 1;
+        p.cols = 16 * ct;
+        // (all passes side by side where that is one round and most of them have work: 40 tokens in tiles of 32 behind 100 11 us, with as many workgroups as the average wants 18)
+        const int average = (int) ((cols + p.cols - 1) / p.cols);
+        p.passes = (R * a.tile_tokens + p.cols - 1) / p.cols;
+        p.launched = ct > 1 && (average * 2 <= p.passes || tiles * p.passes > FEW_WANT) ? average : p.passes;
+        const int64_t slots = tiles * p.passes, busy = tiles * p.launched;
+        p.splits = splits_of(a, pages, slots, busy, FEW_WANT, FEW_LEAST, FEW_MOST, p.cols * (D + 2));
+        if ((pages - (pages + p.splits - 1) / p.splits - 2) * D < FEW_JOIN) p.splits = 1;
+        p.groups = busy * p.splits;
+        p.fits = p.groups < 1 << 23;                       // (a launch has fewer than 2^32 threads; that of the joins is small, as splits make one round at the most)
+        return p;
+    }
+    p.cols = TC; p.passes = p.launched = 1;
+    p.splits = splits_of(a, pages, tiles, tiles, nb <= 4 ? TILES_WANT : TILES_WANT / 2, TILES_LEAST, TILES_MOST, TC * (D + 2));
+    if (pages - (tiles * p.splits > TILES_WANT / 2 ? 1.6 : 1.0) * (double) ((pages + p.splits - 1) / p.splits) < 3.0 + (double) (tiles * p.splits) / 54.0) p.splits = 1;
+    p.groups = tiles * p.splits;
+    p.fits = p.groups < 1 << 24;
+    return p;
+}
 
 // columns per workgroup: the joined values of a thread come from about 16 splits
-template <typename T, int D, int COLS> void join(const pm_kv4_cache & c, const pm_kv4_attn & a, int64_t slots, int passes, int splits, hipStream_t st) {
-    const int most = 1024 / D, want = 16384 / (D * splits), each = want < 1 ? 1 : want < most ? want : most;
-    hipLaunchKernelGGL((join_kernel<T, D, COLS>), dim3((unsigned) (slots * ((COLS + each - 1) / each))), dim3(256), join_factors(splits, each) + 4096, st, c, a, passes, splits, each);
+template <typename T, int D, int COLS> void join(const pm_kv4_cache & c, const pm_kv4_attn & a, const pm_kv4_plan & p, hipStream_t st) {
+    const int most = 1024 / D, want = 16384 / (D * p.splits), each = want < 1 ? 1 : want < most ? want : most;
+    const int64_t slots = (int64_t) a.n_tiles * c.G * p.passes;
+    hipLaunchKernelGGL((join_kernel<T, D, COLS>), dim3((unsigned) (slots * ((COLS + each - 1) / each))), dim3(256), join_factors(p.splits, each) + 4096, st, c, a, p.passes, p.splits, each);
 }
-template <typename T, int NB> int launch(const pm_kv4_cache & c, pm_kv4_attn a, hipStream_t st) {
+template <typename T, int NB, int CT> void few(const pm_kv4_cache & c, const pm_kv4_attn & a, const pm_kv4_plan & p, hipStream_t st) {
+    constexpr int D = NB * 32;
+    const auto kern = few_kernel<T, NB, sizeof(T) == 4, CT>;
+    const size_t ring = (size_t) FW * STAGES * pm_step<NB>::BYTES, acc = (size_t) FW * 16 * (D + 4) * 4, lds = ring > acc ? ring : acc;
+    pm_allow_big_lds((const void *) kern, lds);
+    hipLaunchKernelGGL(kern, dim3((unsigned) p.groups), dim3(FW * 64), lds, st, c, a, p.launched, p.passes, p.splits);
+    if (p.splits > 1) join<T, D, 16 * CT>(c, a, p, st);
+}
+template <typename T, int NB> int launch(const pm_kv4_cache & c, const pm_kv4_attn & a, hipStream_t st) {
     constexpr int D = NB * 32;
     constexpr bool WIDE = sizeof(T) == 4;
-    const int R = a.H / c.G;
-    if (a.window > 0) { const int64_t most = (int64_t) a.window + a.tile_tokens + 128 + a.first; if (most < a.max_keys) a.max_keys = (int) most; }
-    const int64_t pages = ((int64_t) a.max_keys + PM_PAGE - 1) / PM_PAGE;
-    // columns of a tile on the average: tile_tokens only bounds them
-    const int64_t cols = (int64_t) R * (a.n_tokens / a.n_tiles < a.tile_tokens ? (a.n_tokens + a.n_tiles - 1) / a.n_tiles : a.tile_tokens);
-    auto few = [&](auto kern, auto ctc) -> int {
-        constexpr int ct = decltype(ctc)::value;
-        // (all passes side by side where that is one round and most of them have work: 40 tokens in tiles of 32 behind 100 11 us, with as many workgroups as the average wants 18)
-        const int passes = (R * a.tile_tokens + 16 * ct - 1) / (16 * ct), average = (int) ((cols + 16 * ct - 1) / (16 * ct));
-        const int launched = ct > 1 && (average * 2 <= passes || (int64_t) a.n_tiles * c.G * passes > FEW_WANT) ? average : passes;
-        const int64_t slots = (int64_t) a.n_tiles * c.G * passes, busy = (int64_t) a.n_tiles * c.G * launched;
-        int splits = splits_of(a, slots, busy, FEW_WANT, FEW_LEAST, FEW_MOST, 16 * ct * (D + 2));
-        if ((pages - (pages + splits - 1) / splits - 2) * D < FEW_JOIN) splits = 1;
-        if (busy * splits >= 1 << 23 || slots >= 1 << 20) return PM355_E_SHAPE;      // (a launch has fewer than 2^32 threads, that of the joins up to 16 workgroups of 256 per slot)
-        const size_t ring = (size_t) FW * STAGES * pm_step<NB>::BYTES, acc = (size_t) FW * 16 * (D + 4) * 4, lds = ring > acc ? ring : acc;
-        pm_allow_big_lds((const void *) kern, lds);
-        hipLaunchKernelGGL(kern, dim3((unsigned) (busy * splits)), dim3(FW * 64), lds, st, c, a, launched, passes, splits);
-        if (splits > 1) join<T, D, 16 * ct>(c, a, slots, passes, splits, st);
+    const pm_kv4_plan p = plan_of(NB, WIDE, c, a);
+    if (!p.fits) return PM355_E_SHAPE;
+    if (p.cols != TC) {
+        if constexpr (columns_of(NB, WIDE) == 2) if (p.cols == 32) { few<T, NB, 2>(c, a, p, st); return 0; }
+        few<T, NB, 1>(c, a, p, st);
         return 0;
-    };
-    constexpr int CT = NB <= (WIDE ? 3 : 4) ? 2 : 1;
-    const int64_t tiles = (int64_t) a.n_tiles * c.G;
-    if (a.tile_tokens == 1 || cols <= FEW_COLS || (tiles * ((cols + 16 * CT - 1) / (16 * CT)) <= FEW_WANT && tiles * pages <= FEW_PAGES)) {
-        if constexpr (CT == 2) if (cols > 16) return few(few_kernel<T, NB, WIDE, 2>, std::integral_constant<int, 2>());
-        return few(few_kernel<T, NB, WIDE, 1>, std::integral_constant<int, 1>());
     }
-    const int64_t slots = (int64_t) a.n_tiles * c.G;
-    int splits = splits_of(a, slots, slots, NB <= 4 ? TILES_WANT : TILES_WANT / 2, TILES_LEAST, TILES_MOST, TC * (D + 2));
-    if (pages - (slots * splits > TILES_WANT / 2 ? 1.6 : 1.0) * (double) ((pages + splits - 1) / splits) < 3.0 + (double) (slots * splits) / 54.0) splits = 1;
     const size_t lds = 2 * ((size_t) PM_PAGE * (D * 2 + 16) + D * (PM_PAGE * 2 + 16));
-    if (slots * splits >= 1 << 24 || (splits > 1 && slots >= 1 << 17)) return PM355_E_SHAPE;
     static_assert(2 * (PM_PAGE * (D * 2 + 16) + D * (PM_PAGE * 2 + 16)) >= TC * (D + 4) * 4, "the partial sums go through the pages' LDS");
     pm_allow_big_lds((const void *) tiles_kernel<T, NB, WIDE>, lds);
-    hipLaunchKernelGGL((tiles_kernel<T, NB, WIDE>), dim3((unsigned) slots, splits), dim3(256), lds, st, c, a, splits);
-    if (splits > 1) join<T, D, TC>(c, a, slots, 1, splits, st);
+    hipLaunchKernelGGL((tiles_kernel<T, NB, WIDE>), dim3((unsigned) (a.n_tiles * (int64_t) c.G), p.splits), dim3(256), lds, st, c, a, p.splits);
+    if (p.splits > 1) join<T, D, TC>(c, a, p, st);
     return 0;
 }
 
@@ -744,6 +757,7 @@ template <typename T, int NB> int launch(const pm_kv4_cache & c, pm_kv4_attn a, 
 
 // (slots * splits < want + slots, and slots < want where there are splits)
 size_t pm_kv4_work_floats(int H, int G, int d) { return (size_t) 2 * TILES_WANT * TC * (d + 2); }
+pm_kv4_plan pm_attn_kv4_plan(const pm_kv4_cache & c, const pm_kv4_attn & a) { return plan_of(c.d / 32, a.type != PM_BF16, c, a); }
 int pm_launch_attn_kv4(const pm_kv4_cache & c, const pm_kv4_attn & a, hipStream_t st) {
 #define PM_CALL(NB) return a.type == PM_BF16 ? launch<uint16_t, NB>(c, a, st) : launch<float, NB>(c, a, st)
     switch (c.d) { case 64: PM_CALL(2); case 96: PM_CALL(3); case 128: PM_CALL(4); case 192: PM_CALL(6); case 256: PM_CALL(8); }

@@ -22,6 +22,22 @@ static const char * wrong(const pm355_kv4_cache * c) {
     return aligned(c->pages, 16) ? nullptr : "pages are not 16-byte aligned";
 }
 static pm_kv4_cache cache_of(const pm355_kv4_cache * c) { return {c->n_head_kv, c->head_dim, c->n_pages, (char *) c->pages, c->d_table, c->table_ld, c->n_seq}; }
+// the launch's arguments of a call of attn_kv4, or the code of what is wrong with it
+static int attn_of(const pm355_kv4_cache * c, const pm355_attn_kv4_args * p, pm_kv4_attn & a) {
+    if (const char * w = wrong(c)) return fail(PM355_E_SHAPE, w);
+    const int64_t d = c->head_dim;
+    if (!p || !known(p->type)) return fail(PM355_E_UNSUPPORTED, "attn_kv4: type");
+    a = {p->type, p->n_head, p->q, p->ldq, p->out, p->ldo, p->scale, p->window, p->n_first, p->d_tiles, p->n_tiles, p->tile_tokens, p->max_keys, p->n_tokens, p->work, p->work ? p->work_floats : 0};
+    if (p->n_tiles == 0) return 0;
+    if (p->n_tiles < 0 || p->n_tokens < 1 || p->n_head < 1 || p->n_head % c->n_head_kv || !p->q || !p->out || !p->d_tiles || p->ldq < p->n_head * d || p->ldo < p->n_head * d || p->n_head * d > 0x0fffffff ||
+        p->window < 0 || p->n_first < 0 || p->max_keys < 0)
+        return fail(PM355_E_SHAPE, "attn_kv4: shape");
+    if (p->tile_tokens < 1 || (p->tile_tokens > 1 && (int64_t) p->n_head / c->n_head_kv * p->tile_tokens > 128)) return fail(PM355_E_SHAPE, "attn_kv4: tile_tokens");
+    if (!isfinite(p->scale)) return fail(PM355_E_RANGE, "attn_kv4: scale");
+    if ((int64_t) p->n_tiles * p->tile_tokens > 0x7fffffff) return fail(PM355_E_SHAPE, "attn_kv4: n_tiles");
+    if (p->ldq % 8 || p->ldo % 8 || !aligned(p->q, 16) || !aligned(p->out, 16) || !aligned(p->d_tiles, 16) || !aligned(p->work, 16)) return fail(PM355_E_ALIGN, "attn_kv4: rows");
+    return 0;
+}
 
 extern "C" {
 
@@ -70,20 +86,20 @@ size_t pm355_attn_kv4_work_floats(int n_head, int n_head_kv, int head_dim) {
     return n_head_kv > 0 && n_head > 0 && n_head % n_head_kv == 0 && pm_kv4_dim(head_dim) ? pm_kv4_work_floats(n_head, n_head_kv, head_dim) : 0;
 }
 int pm355_attn_kv4(const pm355_kv4_cache * c, const pm355_attn_kv4_args * p, pm355_stream_t st) {
-    if (const char * w = wrong(c)) return fail(PM355_E_SHAPE, w);
-    const int64_t d = c->head_dim;
-    if (!p || !known(p->type)) return fail(PM355_E_UNSUPPORTED, "attn_kv4: type");
-    if (p->n_tiles == 0) return 0;
-    if (p->n_tiles < 0 || p->n_tokens < 1 || p->n_head < 1 || p->n_head % c->n_head_kv || !p->q || !p->out || !p->d_tiles || p->ldq < p->n_head * d || p->ldo < p->n_head * d || p->n_head * d > 0x0fffffff ||
-        p->window < 0 || p->n_first < 0 || p->max_keys < 0)
-        return fail(PM355_E_SHAPE, "attn_kv4: shape");
-    if (p->tile_tokens < 1 || (p->tile_tokens > 1 && (int64_t) p->n_head / c->n_head_kv * p->tile_tokens > 128)) return fail(PM355_E_SHAPE, "attn_kv4: tile_tokens");
-    if (!isfinite(p->scale)) return fail(PM355_E_RANGE, "attn_kv4: scale");
-    if ((int64_t) p->n_tiles * p->tile_tokens > 0x7fffffff) return fail(PM355_E_SHAPE, "attn_kv4: n_tiles");
-    if (p->ldq % 8 || p->ldo % 8 || !aligned(p->q, 16) || !aligned(p->out, 16) || !aligned(p->d_tiles, 16) || !aligned(p->work, 16)) return fail(PM355_E_ALIGN, "attn_kv4: rows");
+    pm_kv4_attn a;
+    if (const int rc = attn_of(c, p, a)) return rc;
+    if (a.n_tiles == 0) return 0;
     (void) hipGetLastError();
-    return done(pm_launch_attn_kv4(cache_of(c), {p->type, p->n_head, p->q, p->ldq, p->out, p->ldo, p->scale, p->window, p->n_first, p->d_tiles, p->n_tiles, p->tile_tokens, p->max_keys, p->n_tokens,
-                                                 p->work, p->work ? p->work_floats : 0}, (hipStream_t) st), "attn_kv4");
+    return done(pm_launch_attn_kv4(cache_of(c), a, (hipStream_t) st), "attn_kv4");
+}
+int pm355_attn_kv4_plan(const pm355_kv4_cache * c, const pm355_attn_kv4_args * p, int32_t * out4) {
+    pm_kv4_attn a;
+    if (!out4) return fail(PM355_E_SHAPE, "attn_kv4_plan: out4");
+    if (const int rc = attn_of(c, p, a)) return rc;
+    const pm_kv4_plan pl = a.n_tiles ? pm_attn_kv4_plan(cache_of(c), a) : pm_kv4_plan{0, 0, 0, 0, 0, true};
+    if (!pl.fits) return fail(PM355_E_SHAPE, "attn_kv4: n_tiles");
+    out4[0] = pl.cols; out4[1] = pl.launched; out4[2] = pl.splits; out4[3] = (int32_t) pl.groups;
+    return 0;
 }
 
 int pm355_pages_copy(void * pages, size_t page_bytes, size_t layer_bytes, int n_layers, int n_pages, const int32_t * pairs, int n_pairs, pm355_stream_t st) {

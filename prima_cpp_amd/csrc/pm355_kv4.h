@@ -24,6 +24,10 @@ struct pm_kv4_attn {
 };
 int pm_launch_kv4_append(const pm_kv4_cache & c, const pm_kv4_append & a, hipStream_t st);
 int pm_launch_kv4_load(const pm_kv4_cache & c, const int32_t * pos, const int32_t * seq, int T, void * k, void * v, hipStream_t st);
+// what a call launches: columns of a workgroup (16, 32: few_kernel, 128: tiles_kernel), passes over the columns of a tile and how many of them start side by side, workgroups that share the keys of
+// one, workgroups in all and whether a launch takes so many
+struct pm_kv4_plan { int cols, passes, launched, splits; int64_t groups; bool fits; };
+pm_kv4_plan pm_attn_kv4_plan(const pm_kv4_cache & c, const pm_kv4_attn & a);
 int pm_launch_attn_kv4(const pm_kv4_cache & c, const pm_kv4_attn & a, hipStream_t st);
 size_t pm_kv4_work_floats(int H, int G, int d);
 int pm_launch_pages_copy(char * pages, size_t page_bytes, size_t layer_bytes, int n_layers, const int32_t * pairs, int n_pairs, hipStream_t st);

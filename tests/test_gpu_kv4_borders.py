@@ -104,3 +104,23 @@ def test_tiles_without_tokens(R):
         ops.attn_kv4(q, dev(raw), dev(table), tiles, tile, 9000, H, G, d, 0.125, out=out, work=work)
         A.compare(out[:1], *A.expected(q[:1], raw, table, [(0, 8999, 1)], H, G, d, 0.125))
         assert (out[1:] == 5.0).all() and (work[1 << 21:] == 7.0).all()
+
+
+def test_very_many_tiles():
+    """131073 rows of 8 KV heads, each a tile: more than 2^20 workgroups"""
+    H = G = 8
+    d, r = 64, np.random.default_rng(0)
+    entries = [(s, 0, 200) for s in range(4)]
+    table, n = tables([200] * 4, r)
+    raw = random_pages(n, G, d, r)
+    at = np.array([(i, 1, i % 200, i // 200) for i in range(800)], np.int32)
+    q = torch.randn(800, H * d, device="cuda").bfloat16()
+    few = ops.attn_kv4(q, dev(raw), dev(table), dev(at), 1, 200, H, G, d, 0.125)
+    A.compare(few, *A.expected(q, raw, table, entries, H, G, d, 0.125))
+    N = (1 << 17) + 1
+    which = np.arange(N) % 800
+    many = at[which]
+    many[:, 0] = np.arange(N)
+    rows = torch.from_numpy(which).cuda()
+    out = ops.attn_kv4(q[rows], dev(raw), dev(table), dev(many), 1, 200, H, G, d, 0.125, work=ops.kv4_work(H, G, d))
+    assert torch.equal(out, few[rows])
