@@ -755,8 +755,8 @@ template <typename T, int NB> int launch(const pm_kv4_cache & c, const pm_kv4_at
 
 } // namespace
 
-// (slots * splits < want + slots, and slots < want where there are splits)
-size_t pm_kv4_work_floats(int H, int G, int d) { return (size_t) 2 * TILES_WANT * TC * (d + 2); }
+// (slots * splits * columns is 128 times what prompts want at the most: few columns have 256 workgroups of up to 32, and up to four times as many slots as workgroups for them)
+size_t pm_kv4_work_floats(int H, int G, int d) { return (size_t) (d <= 128 ? TILES_WANT : TILES_WANT / 2) * TC * (d + 2); }
 pm_kv4_plan pm_attn_kv4_plan(const pm_kv4_cache & c, const pm_kv4_attn & a) { return plan_of(c.d / 32, a.type != PM_BF16, c, a); }
 int pm_launch_attn_kv4(const pm_kv4_cache & c, const pm_kv4_attn & a, hipStream_t st) {
 #define PM_CALL(NB) return a.type == PM_BF16 ? launch<uint16_t, NB>(c, a, st) : launch<float, NB>(c, a, st)
