@@ -1,10 +1,12 @@
-"""The launches of attention over the 4-bit cache: limits, scratch."""
+"""The launches of attention over the 4-bit cache: limits, scratch, which kernel the prompts of the device tests take."""
 import ctypes as C
 import random
 
 import pytest
 
-from kv4_plan import raw_plan
+import test_gpu_kv4_borders as borders
+import test_gpu_kv4_prompts as prompts
+from kv4_plan import plan, raw_plan
 from prima_cpp_amd import lib as L
 
 SHAPE = -2
@@ -41,3 +43,13 @@ def test_scratch_is_what_splits_want(d, type):
         assert used <= n
         most = max(most, used)
     assert most == floats(8, 8, d) == (512 if d <= 128 else 256) * 128 * (d + 2)
+
+
+@pytest.mark.parametrize("type", ["bf16", "f32"])
+@pytest.mark.parametrize("d", [64, 96, 128, 192, 256])
+def test_prompts_of_the_device_tests_are_prompts(d, type):
+    """tests/test_gpu_kv4_prompts.py's cases go to the kernel of 128 columns with any window, some of them with split keys and some without"""
+    splits = {plan(type, *prompts.CASES[c][:2], d, prompts.CASES[c][2], w, f, work) for c in prompts.CASES for w, f in prompts.WINDOWS + [(300, 9), (40, 6), (100, 5), (30, 6)] for work in (True, False)}
+    assert {p[0] for p in splits} == {128} and {p[2] > 1 for p in splits} == {True, False}
+    assert plan(type, 16, 16, d, borders.BATCHES["prompt"])[0] == 128 and all(plan(type, 16, 16, d, e)[0] < 128 for b, e in borders.BATCHES.items() if b != "prompt")
+    assert plan(type, 16, 16, d, borders.BATCHES["far"])[2] > 1
