@@ -488,11 +488,11 @@ PM355_API int pm355_kv4_load(const pm355_kv4_cache * c, const int32_t * d_pos, c
  * bits, so that a position of 10^6 still has its angle to 10^-9. */
 PM355_API int pm355_rope_turns(const pm355_rope_params * rp, const float * freq_factors, double * turns, float * mscale);
 /* Attention over the pages: a query at position i sees the cached keys j <= i, with window > 0 those with i - j < window or j < n_first, on pages that are held; score = scale (q . k) with a finite scale, softmax,
- * weighted values; 0 for a query that sees nothing (position < 0 among them). Queries come in tiles of consecutive tokens of one sequence, device int32 {row, tokens, position of the first,
+ * weighted values; 0 for a query that sees nothing (position < 0 among them), NaN for one that is not finite and sees a key. Queries come in tiles of consecutive tokens of one sequence, device int32 {row, tokens, position of the first,
  * sequence} each, of at most tile_tokens tokens. n_head / n_head_kv * tile_tokens <= 16, or tile_tokens == 1: decoded and drafted tokens, keys split over workgroups by max_keys (the
  * most keys that a tile sees; only the speed depends on it); up to 128: prompts. Keys and values are the cache's f16 values; queries and probabilities are f16 with type BF16 (queries
- * scaled by a power of two per row) and pairs of f16 - 22 bits - with type F32; sums and softmax in f32. work: f32 scratch for split keys, 16-byte aligned, of any size (pm355_attn_kv4_work_floats()
- * lets every split happen) and with any contents, used by one call at a time - graphs captured with the same scratch do not run at once; NULL: no splits. out may be q. Rows that no tile
+ * scaled by a power of two per row) and pairs of f16 - 22 bits - with type F32; sums and softmax in f32. work: f32 scratch for split keys, 16-byte aligned, of any size (pm355_attn_kv4_work_floats(),
+ * up to 34 MB, lets every split happen) and with any contents, used by one call at a time - graphs captured with the same scratch do not run at once; NULL: no splits. out may be q. Rows that no tile
  * names are left as they are. */
 typedef struct {
     int32_t type, n_head; const void * q; int64_t ldq; void * out; int64_t ldo;      /* rows of n_head d values, ld a multiple of 8, 16-byte aligned */
@@ -600,7 +600,7 @@ PM355_API int pm355_page_pool_open(pm355_page_pool * p);                        
 PM355_API int pm355_page_pool_close(pm355_page_pool * p, int seq);
 PM355_API int pm355_page_pool_grow(pm355_page_pool * p, int seq, int n_tokens);           /* pages for positions [0, n_tokens) that are not there yet; all or nothing */
 PM355_API int pm355_page_pool_drop_before(pm355_page_pool * p, int seq, int position);    /* releases the pages that lie wholly in front of `position` */
-PM355_API int pm355_page_pool_drop(pm355_page_pool * p, int seq, int from, int to);       /* releases the pages that lie wholly in [from, to), e.g. between first tokens and window */
+PM355_API int pm355_page_pool_drop(pm355_page_pool * p, int seq, int from, int to);       /* releases the pages that lie wholly in [from, to), e.g. between first tokens and window; these positions get no page again (grow adds behind the last page that there was) */
 /* Forked sequences share pages, which are written by one user only: own() gives `seq` pages of its own from position `from` on and writes (from, to) pairs of what pm355_pages_copy has
  * to copy before the next append; compact() moves the pages in use to the front of the pool. Both return the number of pairs, and change nothing where an error comes back (E_RANGE: more
  * than max_pairs, E_NOMEM: no free pages). */

@@ -2,13 +2,15 @@
 //
 // o = sum_j p_j v_j / sum_j p_j, p_j = exp2(cf q k_j - max), over the j that the query sees; one pass over the keys with the running maximum and sum, both products on the f16 matrix cores.
 // Keys and values become f16 on their way to the products: a pair of codes is masked out of a word over the bits of 1024, less 1032, times the scale - 3.25 operations for two values (the words are
-// ordered so that a mask gives a pair that an operand wants). Queries are brought to [1, 2) by a power of two per row, exact for bf16; WIDE (32-bit rows) holds queries and probabilities as
-// pairs of f16 and makes two products of each. Probabilities are held times 2^8, so that f16 has its steps of 2^-11 down to p = 2^-22.
+// ordered so that a mask gives a pair that an operand wants). Queries are brought to [1, 2) by a power of two per row: exact for bf16 values down to 2^-17 of their row's largest, smaller ones are off
+// by 2^-25 of it at most (f16's last step). Probabilities are held times 2^8, so that f16 has its steps of 2^-11 down to p = 2^-22. With bf16 rows they are single f16, an eighth of the step of the
+// output that they make: the error of long and prompt attention against 64 bits is 0.00166 .. 0.00168 of the values, 0.00165 .. 0.00167 of it the output's own rounding; as pairs of f16 a prompt of
+// 4096 tokens would take 406 us instead of 322 (in a graph), 48 tokens 89 instead of 84. WIDE (32-bit rows) holds queries and probabilities as pairs and makes two products of each.
 // S^T = K Q^T is computed with the key rows permuted so that a lane's score registers are its P operand of O^T = V^T P^T.
 //   few    16 or 32 columns (tokens x query heads of a KV head) per workgroup, 32 keys per wave and step, keys split over waves and workgroups: bound by memory, short prompt portions by the way
 //          through one step. 48 tokens of 64 heads behind 3300 .. 8203 keys 74 us (329 MB, 4.4 TB/s), one of 32 heads behind 131100 37 us (151 MB), 16 x 4 of 28 heads in a window of 4096 24 us; a large copy reaches 4.9 TB/s here
 //   tiles  128 columns per workgroup, a page at a time through LDS, where it is made f16 once for all four waves: bound by the matrix cores, which run at 1.1 .. 1.3 PFLOP/s under load.
-//          4096 tokens of 32 heads behind 2011: 316 us, 860 TFLOP/s (a large f16 product of the library 1110)
+//          4096 tokens of 32 heads behind 2011: 311 .. 318 us, 857 .. 876 TFLOP/s (a large f16 product of the library 1110). 32-bit rows of 256 spill 88 registers: 512 tokens of 16 + 4 heads 63 us, bf16 37
 //   join   the partial sums of split keys
 #include "pm355_kv4.h"
 #include "pm355_kernels.h"
@@ -676,7 +678,8 @@ template <typename T, int D, int COLS> __global__ __launch_bounds__(256) void jo
 // FEW_WANT: one workgroup of 8 waves per CU is enough to fill the memory's queues, and every split costs its join. 32 tokens of 8 KV heads behind 8190 keys: 256 workgroups 67 us, 512 73, 1024 (of
 // 4 waves) 80; one token behind 262100: 72, 72, 82. FEW_COLS: up to there rows of keys are read again per 32 columns; 8 x 16 tokens x 4 heads behind 4000 34 us, as one tile of 128 columns 38.
 // FEW_PAGES: wider tiles go that way too where their workgroups are one round and all of them together read no more pages than this. 64, 128, 256 tokens of 32 + 8 heads of 128: behind 500 16, 19,
-// 16 us, as tiles 23, 24, 28; behind 2000 21, 26, 30 and 26, 29, 34; behind 4000 (1040, 2080, 4224 pages) 25, 34, 46 and 27, 31, 43. 512 tokens (512 workgroups) 26 us, as tiles 21.
+// 16 us, as tiles 23, 24, 28; behind 2000 (528, 1088, 2304 pages) 21, 26, 30 and 26, 29, 34; behind 4000 (1040, 2080, 4224 pages) 25, 34, 46 and 27, 31, 43. 512 tokens (512 workgroups) 26 us, as tiles
+// 21. (No number of pages parts all of these: 256 tokens behind 2000 go the slower way, by 4 us.)
 // FEW_JOIN: a join costs as much as FEW_JOIN / d + 2 pages of a workgroup, which the splits have to save. One token of 8 KV heads of 128 behind 500, 700, 1000, 1500: 9.0, 10.4, 11.7, 14.7 us in one,
 // 11.4 .. 11.5 split; of 64: 7.4, 8.3, 9.2, 11.2 and 10.5 .. 10.8; of 256: 12.7, 15.1, 17.1, 21.4 and 13.7 .. 14.0.
 // TILES_WANT: two workgroups per CU (one from heads of 192 on) share its matrix cores: 1.6 times the time of one, not 2. 512 tokens of 32 + 8 heads of 128 behind 12000 147 us, with 256 167. Partial sums
