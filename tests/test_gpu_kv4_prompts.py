@@ -19,9 +19,8 @@ CASES = {
     "grouped": (8, 2, [(0, 300, 1100), (1, 0, 65)]),                         # tiles of 32 tokens, split keys
     "seven": (14, 2, [(0, 63, 700), (1, 64, 1), (2, 5, 100)]),               # 126 of 128 columns
     "forty": (40, 1, [(0, 190, 301)]),                                       # three tokens a tile
-    "one": (1, 1, [(0, 0, 33000)]),                                          # (a single head: only the last keys are read, see WINDOWED)
+    "one": (1, 1, [(0, 0, 33000)]),                                          # a single head and many tiles
 }
-WINDOWED = {"one"}                                                           # cases that are run with windows alone, for the reference's sake
 WINDOWS = [(0, 0), (1, 0), (7, 64), (64, 0), (100, 130), (200, 17)]
 
 
